@@ -116,6 +116,10 @@ def _load() -> C.CDLL:
         "basalt_k_matmul_f16_allgather": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, P(vp), C.c_int, vp, vp]),
         "basalt_k_fill": (C.c_int, [C.c_int, u64, u64, i64, vp, vp]),
         "basalt_k_matmul_f16_variant": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, P(vp), C.c_int, vp, vp]),
+        "basalt_k_rms_norm": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, i64, vp, C.c_float, vp, i64, vp, i64, i64, vp]),
+        "basalt_k_quantize_e4m3": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, i64, i64, vp]),
+        "basalt_k_matmul_e4m3": (C.c_int, [vp, i64, vp, vp, i64, vp, C.c_int, vp, i64, C.c_int, C.c_int, C.c_int, vp, vp]),
+        "basalt_k_matmul_w4": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, vp, C.c_int, vp, i64, C.c_int, C.c_int, C.c_int, vp, vp]),
         "basalt_k_max_i32_allreduce": (C.c_int, [vp, i64, vp, P(u64), C.c_int, C.c_int, C.c_uint32, vp, vp, vp, u64, vp]),
         "basalt_k_peer_allreduce_max_i32": (C.c_int, [P(u64), C.c_int, C.c_int, C.c_uint32, vp, vp, vp, u64, C.c_int, C.c_int32, vp]),
     }

@@ -21,8 +21,9 @@ CLI = os.path.join(HERE, "basalt-b200")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 CXX_SOURCES = ["bir.cpp", "passes.cpp", "emit.cpp", "emit_mma.cpp", "regbudget.cpp", "frontend_c.cpp", "frontend_triton.cpp", "capi.cpp", "runtime.cpp"]
-CU_SOURCES = ["kernels/common.cu", "kernels/streaming.cu", "kernels/sgemm.cu", "kernels/matmul_f16_tc.cu", "kernels/collective.cu", "kernels/workload_fill.cu"]
-HEADERS = ["bir.hpp", "passes.hpp", "emit.hpp", "frontend_c.hpp", "frontend_triton.hpp", "kernels/common.cuh", "../../include/basalt_b200.h",
+CU_SOURCES = ["kernels/common.cu", "kernels/streaming.cu", "kernels/sgemm.cu", "kernels/matmul_f16_tc.cu", "kernels/collective.cu", "kernels/workload_fill.cu", "kernels/rows_e4m3.cu",
+              "kernels/matmul_e4m3.cu", "kernels/matmul_w4.cu"]
+HEADERS = ["bir.hpp", "passes.hpp", "emit.hpp", "frontend_c.hpp", "frontend_triton.hpp", "kernels/common.cuh", "kernels/tensor_core.cuh", "../../include/basalt_b200.h",
            "../../include/basalt_b200_kernels.h"]
 CXXFLAGS = ["-std=c++17", "-O2", "-fPIC", "-Wall", "-Wextra", "-fvisibility=hidden", f"-I{CUDA_HOME}/include"]
 NVCCFLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler",

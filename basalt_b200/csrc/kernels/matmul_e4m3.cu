@@ -1,0 +1,222 @@
+// e4m3 matmul with row scales for sm_100a:
+//
+//   C[m, n] = (sum_k A[m, k] * B[n, k]) * a_scales[m] * b_scales[n]
+//
+// A [M x K] and B [N x K] are e4m3 rows, the sums f32 in tensor memory (tcgen05.mma.kind::f8f6f4), the product with the
+// two scales and the one rounding to C's type in the epilogue. Rows of B (a layer's weights) lie along the MMA's 128
+// accumulator lanes and rows of A (tokens) along its columns, so one token costs a 16-column tile, not a 128-row one.
+//
+// A CTA computes 128 rows of B x TN rows of A over its share of K: thread 0 of warp 0 feeds a ring of shared-memory
+// stages (128 bytes of K each) by bulk-tensor loads, thread 0 of warp 1 issues the MMAs, and all four warps drain
+// the accumulator. Where there are fewer tiles than the GPU has room for, a cluster of up to eight
+// CTAs shares one tile, each taking a run of K slabs: the partial sums meet in distributed shared memory and are added in
+// the order of the CTAs, so the result depends on no race and needs no workspace.
+// Ragged edges are the tensor maps' business: what lies outside a matrix is read as zero.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../../include/basalt_b200_kernels.h"
+#include "common.cuh"
+#include "tensor_core.cuh"
+
+namespace {
+
+using namespace basalt_k::tc;
+
+constexpr int BN = 128, BK = 128, THREADS = 128, B_BYTES = BN * BK, MMA_K = 32;
+
+__device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <int TN>
+__host__ __device__ constexpr int stages_of() { return TN <= 32 ? 5 : TN == 64 ? 4 : 3; }   // at most 96 KB: two CTAs fit an SM
+template <int TN>
+__host__ __device__ constexpr int smem_of() {
+    constexpr int ring = stages_of<TN>() * (B_BYTES + TN * BK), sums = TN * BN * 4;
+    return (ring > sums ? ring : sums) + 1024;
+}
+
+template <class T, int TN>
+__global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
+                                                              const float* __restrict__ a_scales, const float* __restrict__ b_scales, T* __restrict__ C,
+                                                              int64_t ldc, int M, int N, int K, int tiles_n, int32_t* status) {
+    constexpr int STAGES = stages_of<TN>(), A_BYTES = TN * BK, STAGE_BYTES = B_BYTES + A_BYTES;
+    constexpr uint32_t TMEM_COLS = TN < 32 ? 32 : TN;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t gave_up;
+    const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
+    const int tile = blockIdx.x / splits, n0 = tile % tiles_n * BN, m0 = tile / tiles_n * TN;
+    const int slabs = (K - 1) / BK + 1;
+    const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
+
+    if (threadIdx.x == 0) {
+        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;   // an earlier CTA gave up: do not pile on
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        mbar_init(smem_u32(&acc_bar), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_acc = tmem_slot;
+    bool ok = true;
+
+    if (warp == 0 && lane == 0) {
+        for (int i = 0; i < count; i++) {
+            const int s = i % STAGES;
+            ok &= mbar_wait(smem_u32(&empty_bar[s]), ((i / STAGES) & 1) ^ 1, &gave_up);
+            if (!ok) break;
+            const uint32_t fb = smem_u32(&full_bar[s]), b_dst = tiles + s * STAGE_BYTES, a_dst = b_dst + B_BYTES;
+            mbar_expect_tx(fb, STAGE_BYTES);
+            tma_load_2d(b_dst, &map_b, fb, (first + i) * BK, n0);
+            tma_load_2d(a_dst, &map_a, fb, (first + i) * BK, m0);
+        }
+        if (!ok) {   // let the copies already issued land before the CTA can exit
+            const uint64_t t0 = global_ns();
+            while (global_ns() - t0 < 2000000ull) {}
+        }
+    } else if (warp == 1 && lane == 0) {
+        // D = f32 (bits 4-5 = 1), both operands e4m3 (0) and K-major, N/8 in bits 17-22, M/16 in bits 24-28
+        const uint32_t idesc = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(BN >> 4) << 24);
+        for (int i = 0; i < count; i++) {
+            const int s = i % STAGES;
+            ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t b_src = tiles + s * STAGE_BYTES, a_src = b_src + B_BYTES;
+            const uint64_t db = smem_desc(b_src, 16, 1024), da = smem_desc(a_src, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < BK / MMA_K; k++) umma_f8(tmem_acc, db + (uint64_t)(2 * k), da + (uint64_t)(2 * k), idesc, (i | k) != 0);
+            umma_commit(smem_u32(&empty_bar[s]));
+        }
+        umma_commit(smem_u32(&acc_bar));
+    }
+    __syncwarp();
+
+    ok &= mbar_wait(smem_u32(&acc_bar), 0, &gave_up);   // on give-up the drain still runs (warp-uniformly) on whatever TMEM holds
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const int n = n0 + threadIdx.x, tokens = min(TN, M - m0);
+    const uint32_t src = tmem_acc + ((uint32_t)(warp * 32) << 16);
+    const float b_scale = n < N ? b_scales[n] : 0.0f;
+    float* sums = reinterpret_cast<float*>(smem_raw + (tiles - smem_u32(smem_raw)));
+    if (splits > 1) __syncthreads();   // every wait on the ring is over: its memory takes the partial sums
+#pragma unroll 1
+    for (int c = 0; c < TN; c += 16) {
+        if (c >= tokens) break;
+        uint32_t r[16];
+        __syncwarp();   // the load is the whole warp's
+        tmem_load_16(src + (uint32_t)c, r);
+        if (splits > 1) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) sums[(c + j) * BN + threadIdx.x] = __uint_as_float(r[j]);
+        } else if (n < N) {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (c + j < tokens) store_as(C + (m0 + c + j) * ldc + n, __uint_as_float(r[j]) * a_scales[m0 + c + j] * b_scale);
+        }
+    }
+    if (splits > 1) {
+        __syncwarp();
+        cluster_sync_all();
+        if (n < N) {
+            for (int c = split; c < tokens; c += splits) {
+                const uint32_t at = smem_u32(&sums[c * BN + threadIdx.x]);
+                float total = 0.0f;
+                for (int q = 0; q < splits; q++) total += load_cluster_f32(map_to_cta(at, q));
+                store_as(C + (m0 + c) * ldc + n, total * a_scales[m0 + c] * b_scale);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();   // no CTA leaves while another reads its sums
+    }
+    if (!ok && status) atomicExch(status, 1);
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"(TMEM_COLS) : "memory");
+}
+
+struct Args {
+    const void *a, *b;
+    const float *a_scales, *b_scales;
+    void* c;
+    int64_t lda, ldb, ldc;
+    int M, N, K;
+    int32_t* status;
+    cudaStream_t stream;
+};
+
+const char* const WHO = "matmul_e4m3";
+
+template <class T, int TN>
+int launch(const Args& p) {
+    CUtensorMap ma, mb;
+    if (const int rc = make_tensor_map(&mb, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.b, p.N, p.K, p.ldb, BK, BN)) return rc;
+    if (const int rc = make_tensor_map(&ma, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, p.M, p.K, p.lda, BK, TN)) return rc;
+    auto kern = matmul_e4m3_kernel<T, TN>;
+    constexpr int smem = smem_of<TN>();
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return basalt_k::record(e, WHO);
+    const int tiles_n = (p.N - 1) / BN + 1, slabs = (p.K - 1) / BK + 1;
+    const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TN + 1);
+    int splits = 1;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps four slabs
+    while (splits < 8 && tiles * splits * 2 <= 2 * basalt_k::sm_count() && slabs >= splits * 8) splits *= 2;
+    if (tiles * splits > INT32_MAX) return basalt_k::record_msg(1, WHO, "M * N is too large");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * splits));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = p.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return basalt_k::record(cudaLaunchKernelEx(&cfg, kern, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, tiles_n, p.status), WHO);
+}
+
+template <class T>
+int launch_type(const Args& p) {
+    if (p.M <= 16) return launch<T, 16>(p);
+    if (p.M <= 32) return launch<T, 32>(p);
+    if (p.M <= 64) return launch<T, 64>(p);
+    return launch<T, 128>(p);
+}
+
+}  // namespace
+
+extern "C" int basalt_k_matmul_e4m3(const void* A, int64_t lda, const float* a_scales, const void* B, int64_t ldb, const float* b_scales, int c_type, void* C,
+                                    int64_t ldc, int M, int N, int K, int32_t* status, void* stream) {
+    if (c_type != BASALT_K_TYPE_F16 && c_type != BASALT_K_TYPE_BF16 && c_type != BASALT_K_TYPE_F32) return basalt_k::record_msg(1, WHO, "unknown type of C");
+    if (M < 0 || N < 0) return basalt_k::record_msg(1, WHO, "M and N must not be negative");
+    if (K < 1) return basalt_k::record_msg(1, WHO, "K must be at least 1");
+    if (M > 1 << 30 || N > 1 << 30 || K > 1 << 30) return basalt_k::record_msg(1, WHO, "M, N and K must not exceed 2^30");
+    if (!M || !N) return 0;
+    if (!A || !B || !C || !a_scales || !b_scales) return basalt_k::record_msg(1, WHO, "A, B, C and both scales are needed");
+    const int size = c_type == BASALT_K_TYPE_F32 ? 4 : 2;
+    if (((uintptr_t)A | (uintptr_t)B) & 15 || (lda | ldb) & 15) return basalt_k::record_msg(1, WHO, "A and B and their row strides must be multiples of 16 bytes");
+    if (lda < K || ldb < K || ldc < N) return basalt_k::record_msg(1, WHO, "a row stride lies below the row");
+    if (lda >= (int64_t)1 << 31 || ldb >= (int64_t)1 << 31 || ldc >= (int64_t)1 << 31) return basalt_k::record_msg(1, WHO, "a row stride lies above 2^31 - 1");
+    if ((uintptr_t)C % size || ((uintptr_t)a_scales | (uintptr_t)b_scales | (uintptr_t)status) % 4) return basalt_k::record_msg(1, WHO, "C, the scales or the status are not aligned to their elements");
+    const basalt_k::Span c = {C, M, N, ldc, size};
+    if (overlap(c, {A, M, K, lda, 1}) || overlap(c, {B, N, K, ldb, 1}) || overlap(c, {a_scales, 1, M, M, 4}) || overlap(c, {b_scales, 1, N, N, 4}))
+        return basalt_k::record_msg(1, WHO, "C overlaps an input");
+    if (const int rc = basalt_k::check_device_pointers(WHO, {A, a_scales, B, b_scales, C, status})) return rc;
+    const Args p = {A, B, a_scales, b_scales, C, lda, ldb, ldc, M, N, K, status, (cudaStream_t)stream};
+    if (c_type == BASALT_K_TYPE_F16) return launch_type<__half>(p);
+    if (c_type == BASALT_K_TYPE_BF16) return launch_type<__nv_bfloat16>(p);
+    return launch_type<float>(p);
+}

@@ -1,0 +1,336 @@
+// Product with 4-bit weights for sm_100a, for the few rows of a decode step:
+//
+//   C[m, n] = sum_k X[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]
+//
+// X [M x K] and C [M x N] are f16 or bf16; q is four bits, two to a byte along k (even k in the low half); s has X's type,
+// z is an integer (8 where none are given). The weights are read once for all rows of X, and they are what the call
+// costs: N K / 2 bytes.
+//
+// The sum runs on the tensor cores with exact operands: q - z is a small integer, exact in f16 and in bf16, so
+// mma.sync m16n8k16 adds (q - z) * x over a group in f32 and the group's scale multiplies that sum in f32. Nothing but C
+// is rounded to 16 bits. The instruction's order of k is free as long as both operands share it; it is chosen so that one
+// 32-bit word of packed weights (eight k) and one 16-byte load of X (eight k) feed two instructions without a shuffle
+// between threads. (tcgen05.mma would want the unpacked weights back in shared memory: four times the bytes
+// of the packed ones, for at most 32 columns of work.)
+//
+// A CTA takes 128 rows of the weights over its share of K: one warp feeds a ring of stages (256 k) by bulk-tensor loads,
+// eight warps compute (32 rows x half a stage each). A cluster of up to eight CTAs shares a tile's K where tiles are
+// few; the partial sums meet in distributed shared memory and are added in a fixed order.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../../include/basalt_b200_kernels.h"
+#include "common.cuh"
+#include "tensor_core.cuh"
+
+namespace {
+
+using namespace basalt_k::tc;
+
+constexpr int ROWS = 128, SLAB_K = 256, W_BYTES = ROWS * SLAB_K / 2, CONSUMERS = 8, THREADS = 32 * (CONSUMERS + 1);
+constexpr int UNIT_K = 32, X_BOX_K = 32;   // a unit: the 32 k that one 16-byte piece of a weight row holds
+
+template <int NT>
+__host__ __device__ constexpr int x_bytes_of() { return 8 * NT * SLAB_K * 2; }
+template <int NT>
+__host__ __device__ constexpr int stages_of() { return NT == 1 ? 5 : NT == 2 ? 4 : 3; }   // at most 100 KB: two CTAs fit an SM
+template <int NT>
+__host__ __device__ constexpr int smem_of() { return stages_of<NT>() * (W_BYTES + x_bytes_of<NT>()) + 1024; }
+
+__device__ __forceinline__ uint32_t load_shared_u32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint4 load_shared_v4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// (a & mask) | magic in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t magic) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(magic));
+    return d;
+}
+
+// The zero point of a weight row as the two constants that unpacking subtracts, in both halves of a register.
+template <class T>
+struct Zero;
+template <>
+struct Zero<__half> {
+    __half2 low, high;
+    __device__ __forceinline__ void set(int z) {
+        low = __half2half2(__int2half_rn(1024 + z));
+        high = __half2half2(__int2half_rn(-64 - z));
+    }
+};
+template <>
+struct Zero<__nv_bfloat16> {
+    __nv_bfloat162 low;
+    __device__ __forceinline__ void set(int z) { low = __bfloat162bfloat162(__int2bfloat16_rn(128 + z)); }
+};
+
+// Eight packed weights -> q - z as pairs of k: (0, 4), (1, 5), (2, 6), (3, 7). The four bits are put into the mantissa of a
+// power of two (1024 + q in f16, 128 + q in bf16; 1024 + 16 q for the upper half of a byte), and the subtraction is exact.
+__device__ __forceinline__ void unpack(uint32_t w, const Zero<__half>& z, uint32_t (&p)[4]) {
+    const __half2 sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2C00));   // 2^-4
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t lo = and_or(w >> (8 * i), 0x000F000Fu, 0x64006400u), hi = and_or(w >> (8 * i), 0x00F000F0u, 0x64006400u);
+        const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), z.low);
+        const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, z.high);
+        p[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+        p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+}
+__device__ __forceinline__ void unpack(uint32_t w, const Zero<__nv_bfloat16>& z, uint32_t (&p)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t v = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+        const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z.low);
+        p[i] = *reinterpret_cast<const uint32_t*>(&a);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// NT: tiles of eight rows of X. FLUSH: units (32 k) that certainly share a group, 1, 2 or 4.
+template <class T, int NT, int FLUSH, bool ZEROS>
+__global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                               const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C, int64_t ldc,
+                                                               int M, int N, int K, int group, int tiles_n, int32_t* status) {
+    constexpr int STAGES = stages_of<NT>(), TOKENS = 8 * NT, X_BYTES = x_bytes_of<NT>(), STAGE_BYTES = W_BYTES + X_BYTES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
+    __shared__ volatile uint32_t gave_up;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
+    const int tile = blockIdx.x / splits, n0 = tile % tiles_n * ROWS, m0 = tile / tiles_n * TOKENS;
+    const int slabs = (K - 1) / SLAB_K + 1;
+    const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
+
+    if (threadIdx.x == 0) {
+        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), CONSUMERS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    bool ok = true;
+    float total[2][NT][4] = {};
+
+    if (warp == CONSUMERS) {
+        if (lane == 0) {
+            for (int i = 0; i < count; i++) {
+                const int s = i % STAGES;
+                ok &= mbar_wait(smem_u32(&empty_bar[s]), ((i / STAGES) & 1) ^ 1, &gave_up);
+                if (!ok) break;
+                const uint32_t fb = smem_u32(&full_bar[s]), w_dst = ring + s * STAGE_BYTES, x_dst = w_dst + W_BYTES;
+                const int k = (first + i) * SLAB_K;
+                mbar_expect_tx(fb, STAGE_BYTES);
+                tma_load_2d(w_dst, &map_w, fb, k / 2, n0);
+#pragma unroll
+                for (int b = 0; b < SLAB_K / X_BOX_K; b++) tma_load_2d(x_dst + b * TOKENS * X_BOX_K * 2, &map_x, fb, k + b * X_BOX_K, m0);
+            }
+            if (!ok) {   // let the copies already issued land before the CTA can exit
+                const uint64_t t0 = global_ns();
+                while (global_ns() - t0 < 2000000ull) {}
+            }
+        }
+        __syncwarp();
+    } else {
+        const int half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
+        const int groups = (K - 1) / group + 1;
+        const T* scale_row[4];
+        const uint8_t* zero_row[4];
+        bool row_in[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int n = n0 + row0 + g + 8 * r;
+            row_in[r] = n < N;
+            scale_row[r] = scales + (int64_t)(row_in[r] ? n : 0) * groups;
+            zero_row[r] = ZEROS ? zeros + (int64_t)(row_in[r] ? n : 0) * groups : nullptr;
+        }
+        for (int i = 0; i < count; i++) {
+            const int s = i % STAGES;
+            float scale[4 / FLUSH][4];
+            int zero[4 / FLUSH][4];
+#pragma unroll
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                const int which = ((first + i) * SLAB_K + half * 128 + f * FLUSH * UNIT_K) / group;
+                const bool in = which < groups;   // past the end of K: X is zero there, and so is the scale
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    scale[f][r] = in && row_in[r] ? to_float(scale_row[r][which]) : 0.0f;
+                    zero[f][r] = ZEROS && in ? zero_row[r][which] : 8;
+                }
+            }
+            ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t w_at = ring + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
+            const uint32_t x_at = ring + s * STAGE_BYTES + W_BYTES + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
+#pragma unroll
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                float acc[2][NT][4] = {};
+                Zero<T> z[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) z[r].set(zero[f][r]);
+#pragma unroll
+                for (int v = 0; v < FLUSH; v++) {
+                    const int u = f * FLUSH + v;
+                    uint32_t a[4][4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) unpack(load_shared_u32(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), z[r], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        const uint4 x = load_shared_v4(x_at + u * TOKENS * X_BOX_K * 2 + nt * 8 * X_BOX_K * 2);   // row 8 nt + g of X, its k 8 t .. 8 t + 7 of the unit
+                        const uint32_t b0 = __byte_perm(x.x, x.z, 0x5410), b1 = __byte_perm(x.x, x.z, 0x7632);
+                        const uint32_t b2 = __byte_perm(x.y, x.w, 0x5410), b3 = __byte_perm(x.y, x.w, 0x7632);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            mma_16816<T>(acc[h][nt], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], b0, b1);
+                            mma_16816<T>(acc[h][nt], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], b2, b3);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) total[h][nt][j] += scale[f][2 * h + (j >> 1)] * acc[h][nt][j];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
+        }
+    }
+
+    // The two halves of a stage and the CTAs of the cluster, added in that order.
+    __syncthreads();   // the ring is done with: its memory takes the partial sums, [half][row of X][row of the weights]
+    float* sums = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
+    if (warp < CONSUMERS) {
+        float* mine = sums + (warp >> 2) * TOKENS * ROWS + (warp & 3) * 32 + (lane >> 2);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) mine[(8 * nt + 2 * (lane & 3) + (j & 1)) * ROWS + 16 * h + 8 * (j >> 1)] = total[h][nt][j];
+    }
+    cluster_sync_all();
+    const int tokens = min(TOKENS, M - m0);
+    for (int i = threadIdx.x; i < ((tokens - split + splits - 1) / splits) * ROWS; i += THREADS) {
+        const int row = i % ROWS, c = i / ROWS * splits + split;
+        if (n0 + row >= N) continue;
+        const uint32_t at = smem_u32(&sums[c * ROWS + row]);
+        float v = 0.0f;
+        for (int q = 0; q < splits; q++) {
+            const uint32_t theirs = map_to_cta(at, q);
+            v += load_cluster_f32(theirs) + load_cluster_f32(theirs + TOKENS * ROWS * 4);
+        }
+        store_as(C + (m0 + c) * ldc + n0 + row, v);
+    }
+    if (!ok && status) atomicExch(status, 1);
+    __syncwarp();
+    cluster_sync_all();   // no CTA leaves while another reads its sums
+}
+
+struct Args {
+    const void *x, *w, *scales;
+    const uint8_t* zeros;
+    void* c;
+    int64_t ldx, ldw, ldc;
+    int M, N, K, group;
+    int32_t* status;
+    cudaStream_t stream;
+};
+
+const char* const WHO = "matmul_w4";
+
+template <class T, int NT, int FLUSH, bool ZEROS>
+int launch(const Args& p) {
+    CUtensorMap mw, mx;
+    const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
+    if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, X_BOX_K, 8 * NT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    auto kern = matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
+    constexpr int smem = smem_of<NT>();
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return basalt_k::record(e, WHO);
+    const int tiles_n = (p.N - 1) / ROWS + 1, slabs = (p.K - 1) / SLAB_K + 1;
+    const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / (8 * NT) + 1);
+    int splits = 1;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps two slabs
+    while (splits < 8 && tiles * splits * 2 <= 2 * basalt_k::sm_count() && slabs >= splits * 4) splits *= 2;
+    if (tiles * splits > INT32_MAX) return basalt_k::record_msg(1, WHO, "M * N is too large");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * splits));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = p.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return basalt_k::record(
+        cudaLaunchKernelEx(&cfg, kern, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c, p.ldc, p.M, p.N, p.K, p.group, tiles_n, p.status), WHO);
+}
+
+template <class T, int NT, int FLUSH>
+int launch_zeros(const Args& p) { return p.zeros ? launch<T, NT, FLUSH, true>(p) : launch<T, NT, FLUSH, false>(p); }
+
+template <class T, int NT>
+int launch_flush(const Args& p) {
+    const int units = p.group / UNIT_K;
+    return units % 4 == 0 ? launch_zeros<T, NT, 4>(p) : units % 2 == 0 ? launch_zeros<T, NT, 2>(p) : launch_zeros<T, NT, 1>(p);
+}
+
+template <class T>
+int launch_type(const Args& p) { return p.M <= 8 ? launch_flush<T, 1>(p) : p.M <= 16 ? launch_flush<T, 2>(p) : launch_flush<T, 4>(p); }
+
+}  // namespace
+
+extern "C" int basalt_k_matmul_w4(int type, const void* X, int64_t ldx, const void* W, int64_t ldw, const void* scales, const uint8_t* zeros, int group, void* C,
+                                  int64_t ldc, int M, int N, int K, int32_t* status, void* stream) {
+    if (type != BASALT_K_TYPE_F16 && type != BASALT_K_TYPE_BF16) return basalt_k::record_msg(1, WHO, "X must be f16 or bf16");
+    if (M < 0 || N < 0) return basalt_k::record_msg(1, WHO, "M and N must not be negative");
+    if (K < 1) return basalt_k::record_msg(1, WHO, "K must be at least 1");
+    if (M > 1 << 30 || N > 1 << 30 || K > 1 << 30) return basalt_k::record_msg(1, WHO, "M, N and K must not exceed 2^30");
+    if (group < UNIT_K || group % UNIT_K) return basalt_k::record_msg(1, WHO, "the group must be a multiple of 32");
+    if (!M || !N) return 0;
+    if (!X || !W || !C || !scales) return basalt_k::record_msg(1, WHO, "X, W, C and the scales are needed");
+    if (((uintptr_t)X | (uintptr_t)W) & 15 || ldw & 15 || ldx & 7) return basalt_k::record_msg(1, WHO, "X and W and their row strides must be multiples of 16 bytes");
+    if (ldx < K || ldw < ((int64_t)K + 1) / 2 || ldc < N) return basalt_k::record_msg(1, WHO, "a row stride lies below the row");
+    if (ldx >= (int64_t)1 << 31 || ldw >= (int64_t)1 << 31 || ldc >= (int64_t)1 << 31) return basalt_k::record_msg(1, WHO, "a row stride lies above 2^31 - 1");
+    if (((uintptr_t)C | (uintptr_t)scales) % 2 || (uintptr_t)status % 4) return basalt_k::record_msg(1, WHO, "C, the scales or the status are not aligned to their elements");
+    const int64_t groups = (K - 1) / group + 1, packed = ((int64_t)K + 1) / 2;
+    const basalt_k::Span c = {C, M, N, ldc, 2};
+    if (overlap(c, {X, M, K, ldx, 2}) || overlap(c, {W, N, packed, ldw, 1}) || overlap(c, {scales, N, groups, groups, 2}) || overlap(c, {zeros, N, groups, groups, 1}))
+        return basalt_k::record_msg(1, WHO, "C overlaps an input");
+    if (const int rc = basalt_k::check_device_pointers(WHO, {X, W, scales, zeros, C, status})) return rc;
+    const Args p = {X, W, scales, zeros, C, ldx, ldw, ldc, M, N, K, group, status, (cudaStream_t)stream};
+    return type == BASALT_K_TYPE_F16 ? launch_type<__half>(p) : launch_type<__nv_bfloat16>(p);
+}

@@ -165,6 +165,50 @@ int basalt_k_matmul_f16_variant(const void *A, const void *B, void *C, int M, in
 enum { BASALT_K_FILL_U32 = 0, BASALT_K_FILL_I32_PM30 = 1, BASALT_K_FILL_F32_PM1 = 2, BASALT_K_FILL_F16_NORMAL01 = 3 };
 int basalt_k_fill(int kind, uint64_t seed, uint64_t start, int64_t n, void *out, void *stream);
 
+/* ---- A quantised linear layer around the matmul: norm, row quantisation, e4m3 and 4-bit products ----
+ *
+ * Row strides lie below 2^31; M, N and K of the products do not exceed 2^30.  C overlaps no input.
+ * The reference has no counterpart to these four. Element types of matrices and vectors: */
+enum { BASALT_K_TYPE_F16 = 0, BASALT_K_TYPE_BF16 = 1, BASALT_K_TYPE_F32 = 2 };
+
+/* Root-mean-square norm of rows, with a residual's addition before it and a quantisation after it:
+ *   h = x + residual          total = h rounded to `type`         y = h * weight / sqrt(mean_k(h_k^2) + eps)
+ * in f32, for rows x cols matrices of `type` (F16, BF16, F32) whose rows lie ld* elements apart (cols <= ld < 2^31).
+ * residual, total and weight may be NULL (no addition; h not stored; weight 1); total needs residual.
+ * scales NULL: y is of `type`.  scales given: y is e4m3 bytes (rows ldy bytes apart) and scales[r] an f32 with
+ *   scales[r] = max(max_k |y_k| / 448, 2^-126),   y stored as e4m3(y_k / scales[r]), to the nearest, ties to even.
+ * The norm goes by h before its rounding to total.  An infinity or a NaN in a row gives what the formulas give; no other
+ * row is touched by it.  An output may be an input's own buffer of the same stride and type (total = residual, y = x); any
+ * other overlap is refused.  Any alignment and width is right; 16-byte aligned rows of whole 16-byte pieces are read
+ * once, others twice.  rows = 0 does nothing.  Pointers must lie on the current device. */
+int basalt_k_rms_norm(int type, const void *x, int64_t ldx, const void *residual, int64_t ldr, void *total, int64_t ldt,
+                      const void *weight, float eps, void *y, int64_t ldy, float *scales, int64_t rows, int64_t cols,
+                      void *stream);
+
+/* The quantisation alone: scales[r] = max(max_k |x_k| / 448, 2^-126), q = e4m3(x_k / scales[r]); for the activations between
+ * two products, and for weights (rows = output channels).  Arguments as above. */
+int basalt_k_quantize_e4m3(int type, const void *x, int64_t ldx, void *q, int64_t ldq, float *scales, int64_t rows,
+                           int64_t cols, void *stream);
+
+/* C[m, n] = (sum_k A[m, k] * B[n, k]) * a_scales[m] * b_scales[n]: A [M x K] and B [N x K] (weights, one row per output
+ * channel) are e4m3, the sums f32 on tcgen05 tensor cores, C [M x N] is of c_type (F16, BF16, F32), rounded once.  Any M, N, K >= 1
+ * (M or N 0 does nothing); A, B, lda and ldb must be multiples of 16 bytes (pad the rows: bytes
+ * beyond K are not read), C and ldc need their element's alignment only.  Rows and columns beyond M and N are left as
+ * they were.  No workspace, no atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16. */
+int basalt_k_matmul_e4m3(const void *A, int64_t lda, const float *a_scales, const void *B, int64_t ldb,
+                         const float *b_scales, int c_type, void *C, int64_t ldc, int M, int N, int K, int32_t *status,
+                         void *stream);
+
+/* C[m, n] = sum_k X[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]: X [M x K] and C [M x N] of `type` (F16 or
+ * BF16), W the four-bit q, two to a byte along k (k even in the low half), rows ldw bytes apart; scales s [N x
+ * ceil(K / group)] of `type` and zeros z [N x ceil(K / group)] (one byte each, 0 .. 128; NULL: 8 everywhere), both
+ * without gaps.  group is a multiple of 32.  Any M, N, K >= 1 (M or N 0 does nothing); X, W and ldw must be
+ * multiples of 16 bytes, ldx of 8 elements.  Sums are f32, C is rounded once.  No workspace, no atomics.  `status` as for
+ * basalt_k_matmul_f16. */
+int basalt_k_matmul_w4(int type, const void *X, int64_t ldx, const void *W, int64_t ldw, const void *scales,
+                       const uint8_t *zeros, int group, void *C, int64_t ldc, int M, int N, int K, int32_t *status,
+                       void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
