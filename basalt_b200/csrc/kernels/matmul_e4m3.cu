@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../../include/basalt_b200_kernels.h"
 #include "common.cuh"
 #include "tensor_core.cuh"
@@ -29,6 +31,17 @@ constexpr int BN = 128, BK = 128, THREADS = 128, B_BYTES = BN * BK, MMA_K = 32;
 __device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <class T>
+__device__ __forceinline__ uint32_t two_as(float a, float b) {
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
 
 template <int TN>
 __host__ __device__ constexpr int stages_of() { return TN <= 32 ? 5 : TN == 64 ? 4 : 3; }   // at most 96 KB: two CTAs fit an SM
@@ -150,6 +163,183 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"(TMEM_COLS) : "memory");
 }
 
+// ---- many tokens: a pair of CTAs per 256 x 256 tile, tcgen05.mma.cta_group::2 ----
+//
+// Rows of A (tokens) along the accumulator's lanes. CTA r of the pair loads rows 128 r .. of the tile's A and columns 128 r .. of its
+// B, 32 KB a slab of 128 bytes of K, and holds its 128 rows of the accumulator; the even CTA issues every
+// MMA. Persistent: one warp feeds the ring, one issues, four drain the accumulator of the tile before (two of them
+// in tensor memory), so the stores of a tile hide behind the next one's products.
+namespace pair {
+constexpr int TM = 256, TN = 256, HALF = 128, STAGES = 6, STAGE_BYTES = 2 * HALF * BK, PIECE_BYTES = 32 * 128, PAIR_THREADS = 192, GROUP_M = 8;
+constexpr int SMEM = STAGES * STAGE_BYTES + 4 * (PIECE_BYTES + TN * 4) + 1024;
+constexpr uint32_t TMEM_COLS = 512;
+
+// Tiles in bands of GROUP_M tile rows, so that the tiles in flight share panels of A and B in L2.
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* m, int* n) {
+    const int per_band = GROUP_M * tiles_n, band = t / per_band, first = band * GROUP_M, rows = min(GROUP_M, tiles_m - first), r = t - band * per_band;
+    *m = first + r % rows;
+    *n = r / rows;
+}
+
+// VECTORS: C's rows are whole 16-byte pieces from an aligned start.
+template <class T, bool VECTORS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    matmul_e4m3_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const float* __restrict__ a_scales,
+                     const float* __restrict__ b_scales, T* __restrict__ C, int64_t ldc, int M, int N, int K, int32_t* status) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tfull_bar[2], tempty_bar[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t gave_up;
+    const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int tiles_m = (M - 1) / TM + 1, tiles_n = (N - 1) / TN + 1, num_tiles = tiles_m * tiles_n, slabs = (K - 1) / BK + 1;
+
+    if (threadIdx.x == 0) {
+        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1);    // the leader's producer; bytes arrive from both CTAs
+            mbar_init(smem_u32(&empty_bar[s]), 1);   // one commit of the leader's MMA warp
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(smem_u32(&tfull_bar[b]), 1);
+            mbar_init(smem_u32(&tempty_bar[b]), 8);   // four epilogue warps in each CTA (used in the leader only)
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {   // the same warp of both CTAs allocates for the pair
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync_all();   // the peer's barriers are initialised before anything can signal them
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_slot;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0;
+            for (int t = pair; t < num_tiles && ok; t += pairs) {
+                int mi, ni;
+                tile_at(t, tiles_m, tiles_n, &mi, &ni);
+                const int m0 = mi * TM + (int)rank * HALF, n0 = ni * TN + (int)rank * HALF;
+                for (int kb = 0; kb < slabs; kb++) {
+                    ok &= mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
+                    if (!ok) break;
+                    const uint32_t fb_local = smem_u32(&full_bar[s]), fb = map_to_cta(fb_local, 0), a_dst = tiles + s * STAGE_BYTES;
+                    if (leader) mbar_expect_tx(fb_local, 2 * STAGE_BYTES);
+                    tma_load_2d_pair(a_dst, &map_a, fb, kb * BK, m0);
+                    tma_load_2d_pair(a_dst + HALF * BK, &map_b, fb, kb * BK, n0);
+                    if (++s == STAGES) s = 0, ph ^= 1;
+                }
+            }
+            if (!ok) {   // let the copies already issued land before the CTA can exit
+                const uint64_t t0 = global_ns();
+                while (global_ns() - t0 < 2000000ull) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+            uint32_t s = 0, ph = 0, local = 0;
+            for (int t = pair; t < num_tiles && ok; t += pairs, local++) {
+                const uint32_t buf = local & 1, use = local >> 1;
+                ok &= mbar_wait(smem_u32(&tempty_bar[buf]), (use & 1) ^ 1, &gave_up);   // both epilogues have drained this accumulator
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int kb = 0; kb < slabs; kb++) {
+                    ok &= mbar_wait(smem_u32(&full_bar[s]), ph, &gave_up);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t a_src = tiles + s * STAGE_BYTES;
+                    const uint64_t da = smem_desc(a_src, 16, 1024), db = smem_desc(a_src + HALF * BK, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < BK / MMA_K; k++) umma_f8_pair(tmem_base + buf * TN, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb | k) != 0);
+                    umma_commit_pair(smem_u32(&empty_bar[s]));
+                    if (++s == STAGES) s = 0, ph ^= 1;
+                }
+                umma_commit_pair(smem_u32(&tfull_bar[buf]));
+            }
+        }
+    } else {
+        // Each 32-row piece of 128 bytes a row is transposed through shared memory and stored as whole lines.
+        constexpr int COLS = 128 / sizeof(T), W = 16 / sizeof(T);
+        const int ew = warp & 3;   // this warp may touch lanes 32 ew .. 32 ew + 31
+        uint8_t* stage = smem_raw + (tiles - smem_u32(smem_raw)) + STAGES * STAGE_BYTES + ew * PIECE_BYTES;
+        float* scale = reinterpret_cast<float*>(smem_raw + (tiles - smem_u32(smem_raw)) + STAGES * STAGE_BYTES + 4 * PIECE_BYTES) + ew * TN;
+        uint32_t local = 0;
+        for (int t = pair; t < num_tiles && ok; t += pairs, local++) {
+            int mi, ni;
+            tile_at(t, tiles_m, tiles_n, &mi, &ni);
+            const uint32_t buf = local & 1, use = local >> 1;
+            const int m0 = mi * TM + (int)rank * HALF + ew * 32, n0 = ni * TN;
+            const float a_scale = m0 + lane < M ? a_scales[m0 + lane] : 0.0f;
+            __syncwarp();   // the tile before has been read out of `scale`
+#pragma unroll
+            for (int i = 0; i < TN / 32; i++) scale[lane + 32 * i] = n0 + lane + 32 * i < N ? b_scales[n0 + lane + 32 * i] : 0.0f;
+            ok &= mbar_wait(smem_u32(&tfull_bar[buf]), use & 1, &gave_up);
+            ok = __all_sync(0xffffffffu, ok);   // the warp stays together: the loads of tensor memory are warp-collective
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t src = tmem_base + buf * TN + ((uint32_t)(ew * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < TN; c += COLS) {
+#pragma unroll
+                for (int part = 0; part < COLS / 32; part++) {
+                    uint32_t r[32];
+                    tmem_load_32(src + (uint32_t)(c + 32 * part), r);
+#pragma unroll
+                    for (int q = 0; q < 32 / W; q++) {   // 16-byte piece q of this lane's row, at a place rotated by the row: no bank conflicts
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < W; i += 4) {
+                            const float4 b = *reinterpret_cast<const float4*>(scale + c + 32 * part + W * q + i);
+                            const float v0 = __uint_as_float(r[W * q + i]) * a_scale * b.x, v1 = __uint_as_float(r[W * q + i + 1]) * a_scale * b.y;
+                            const float v2 = __uint_as_float(r[W * q + i + 2]) * a_scale * b.z, v3 = __uint_as_float(r[W * q + i + 3]) * a_scale * b.w;
+                            if constexpr (sizeof(T) == 4) w[0] = __float_as_uint(v0), w[1] = __float_as_uint(v1), w[2] = __float_as_uint(v2), w[3] = __float_as_uint(v3);
+                            else w[i / 2] = two_as<T>(v0, v1), w[i / 2 + 1] = two_as<T>(v2, v3);
+                        }
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + (((32 / W * part + q) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+                if (c + COLS == TN) {   // the accumulator is drained: the MMA warp may overwrite it while the stores go out
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[buf]), 0));
+                }
+                const int row = lane >> 3, piece = lane & 7, n = n0 + c + W * piece;   // eight lanes to a row
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int m = m0 + 4 * i + row;
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + (4 * i + row) * 128 + ((piece ^ ((4 * i + row) & 7)) << 4));
+                    T* to = C + m * ldc + n;
+                    if (VECTORS && m < M && n + W <= N) *reinterpret_cast<uint4*>(to) = v;
+                    else if (m < M) {
+                        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                        for (int j = 0; j < W; j++)
+                            if (n + j < N) to[j] = e[j];
+                    }
+                }
+                __syncwarp();   // the next piece may overwrite the staging rows
+            }
+        }
+    }
+    if (!ok && status) atomicExch(status, 1);
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync_all();   // the peer has stopped naming this CTA's barriers, shared and tensor memory
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+}
+}  // namespace pair
+
 struct Args {
     const void *a, *b;
     const float *a_scales, *b_scales;
@@ -188,8 +378,26 @@ int launch(const Args& p) {
     return basalt_k::record(cudaLaunchKernelEx(&cfg, kern, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, tiles_n, p.status), WHO);
 }
 
+template <class T, bool VECTORS>
+int launch_pair(const Args& p) {
+    CUtensorMap ma, mb;
+    if (const int rc = make_tensor_map(&ma, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, p.M, p.K, p.lda, BK, pair::HALF)) return rc;
+    if (const int rc = make_tensor_map(&mb, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.b, p.N, p.K, p.ldb, BK, pair::HALF)) return rc;
+    auto kern = pair::matmul_e4m3_pair<T, VECTORS>;
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM)) return basalt_k::record(e, WHO);
+    const int64_t tiles = (int64_t)((p.M - 1) / pair::TM + 1) * ((p.N - 1) / pair::TN + 1);
+    if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
+    const int pairs = (int)(tiles < basalt_k::sm_count() / 2 ? tiles : basalt_k::sm_count() / 2);
+    kern<<<2 * pairs, pair::PAIR_THREADS, pair::SMEM, p.stream>>>(ma, mb, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, p.status);
+    return basalt_k::record(cudaGetLastError(), WHO);
+}
+
 template <class T>
 int launch_type(const Args& p) {
+    if (p.M > 256) {
+        const bool vectors = (uintptr_t)p.c % 16 == 0 && p.ldc * sizeof(T) % 16 == 0;
+        return vectors ? launch_pair<T, true>(p) : launch_pair<T, false>(p);
+    }
     if (p.M <= 16) return launch<T, 16>(p);
     if (p.M <= 32) return launch<T, 32>(p);
     if (p.M <= 64) return launch<T, 64>(p);
