@@ -50,6 +50,9 @@ __device__ __forceinline__ uint4 load_shared_v4(uint32_t at) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
     return v;
 }
+__device__ __forceinline__ void store_shared_v4(uint32_t at, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
@@ -259,6 +262,267 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     cluster_sync_all();   // no CTA leaves while another reads its sums
 }
 
+// ---- many rows of X: the weights unpacked into shared memory for tcgen05.mma ----
+//
+// The weights lie along the accumulator's 128 lanes and up to 256 rows of X along its columns (the width of a tile is the
+// host's choice, a multiple of 16). Per slab of 64 k eight warps turn 4 KB of packed weights into the 16 KB swizzled tile that
+// the MMA reads, (q - z) * s rounded to X's type: unlike the kernel above, which scales sums, this one scales the operand,
+// because a group's sum would have to leave tensor memory for every group. That is one rounding of half a step a weight, of
+// random sign, beside the one of C: the error of C grows by the root of two.
+// Persistent where there are more tiles than SMs (two accumulators: a tile's stores hide behind the next one's products); a
+// cluster shares a tile's K, as above, where there are fewer.
+namespace tall {
+constexpr int TILE_K = 64, W_TILE = ROWS * TILE_K * 2, RAW_BYTES = W_BYTES, MAX_STAGES = 6, MAX_RAW = 4;
+constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, UNPACKERS = 8, FIRST_UNPACKER = 3 + 1, EPILOGUE = 4, FIRST_EPILOGUE = FIRST_UNPACKER + UNPACKERS;
+constexpr int TALL_THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE), SMEM_MOST = 231936;
+constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 256;
+
+// Eight packed weights of one group -> (q - z) * s in the order of k, two to a register.
+template <class T>
+__device__ __forceinline__ uint4 unpack_scaled(uint32_t w, uint32_t zero, uint32_t scale) {
+    constexpr uint32_t MAGIC = std::is_same_v<T, __half> ? 0x64006400u : 0x43004300u;
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const uint32_t up = w >> 4;
+    uint32_t p[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const uint32_t v = and_or(__byte_perm(w, up, b | (4 + b) << 8), 0x000F000Fu, MAGIC);
+        const T2 a = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&v), *reinterpret_cast<const T2*>(&zero)), *reinterpret_cast<const T2*>(&scale));
+        p[b] = *reinterpret_cast<const uint32_t*>(&a);
+    }
+    return make_uint4(p[0], p[1], p[2], p[3]);
+}
+__device__ __forceinline__ uint32_t zero_of(__half, int z) { return 0x00010001u * __half_as_ushort(__int2half_rn(1024 + z)); }
+__device__ __forceinline__ uint32_t zero_of(__nv_bfloat16, int z) { return 0x00010001u * __bfloat16_as_ushort(__int2bfloat16_rn(128 + z)); }
+
+struct Shape {
+    int M, N, K, group, tile_m, tiles_n, tiles, stages, raws;
+};
+
+template <class T, bool ZEROS>
+__global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                  const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C,
+                                                                  int64_t ldc, const Shape p, int32_t* status) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], raw_full[MAX_RAW], raw_empty[MAX_RAW], tfull_bar[2], tempty_bar[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t gave_up;
+    const uint32_t raw = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = raw + p.raws * RAW_BYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
+    const int my_tile = blockIdx.x / splits, step = gridDim.x / splits;
+    const int slabs = (p.K - 1) / SLAB_K + 1, first = (int)((int64_t)slabs * split / splits), slabs_here = (int)((int64_t)slabs * (split + 1) / splits) - first;
+    const int count = min(slabs_here * (SLAB_K / TILE_K), (p.K - 1) / TILE_K + 1 - first * (SLAB_K / TILE_K));   // tiles of 64 k
+    const int x_bytes = p.tile_m * TILE_K * 2, stage_bytes = W_TILE + x_bytes;
+
+    if (threadIdx.x == 0) {
+        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1 + UNPACKERS);   // the rows of X, and each unpacking warp
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        for (int s = 0; s < p.raws; s++) {
+            mbar_init(smem_u32(&raw_full[s]), 1);
+            mbar_init(smem_u32(&raw_empty[s]), UNPACKERS);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(smem_u32(&tfull_bar[b]), 1);
+            mbar_init(smem_u32(&tempty_bar[b]), EPILOGUE);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == WARP_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_slot;
+    bool ok = true;
+
+    if (warp == WARP_X) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int t = my_tile; t < p.tiles && ok; t += step) {
+                const int m0 = t / p.tiles_n * p.tile_m;
+                for (int i = 0; i < count; i++) {
+                    ok &= mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
+                    if (!ok) break;
+                    const uint32_t fb = smem_u32(&full_bar[s]);
+                    mbar_expect_tx(fb, x_bytes);
+                    tma_load_2d(ring + s * stage_bytes + W_TILE, &map_x, fb, first * SLAB_K + i * TILE_K, m0);
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
+            }
+            if (!ok) {   // let the copies already issued land before the CTA can exit
+                const uint64_t t0 = global_ns();
+                while (global_ns() - t0 < 2000000ull) {}
+            }
+        }
+    } else if (warp == WARP_RAW) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int t = my_tile; t < p.tiles && ok; t += step) {
+                const int n0 = t % p.tiles_n * ROWS;
+                for (int i = 0; i < slabs_here; i++) {
+                    ok &= mbar_wait(smem_u32(&raw_empty[s]), ph ^ 1, &gave_up);
+                    if (!ok) break;
+                    const uint32_t fb = smem_u32(&raw_full[s]);
+                    mbar_expect_tx(fb, RAW_BYTES);
+                    tma_load_2d(raw + s * RAW_BYTES, &map_w, fb, (first + i) * SLAB_K / 2, n0);
+                    if (++s == p.raws) s = 0, ph ^= 1;
+                }
+            }
+            if (!ok) {
+                const uint64_t t0 = global_ns();
+                while (global_ns() - t0 < 2000000ull) {}
+            }
+        }
+    } else if (warp == WARP_MMA) {
+        if (lane == 0) {
+            const uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
+            const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.tile_m >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+            int s = 0;
+            uint32_t ph = 0, local = 0;
+            for (int t = my_tile; t < p.tiles && ok; t += step, local++) {
+                const uint32_t buf = local & 1, use = local >> 1;
+                ok &= mbar_wait(smem_u32(&tempty_bar[buf]), (use & 1) ^ 1, &gave_up);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int i = 0; i < count; i++) {
+                    ok &= mbar_wait(smem_u32(&full_bar[s]), ph, &gave_up);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t w_src = ring + s * stage_bytes;
+                    const uint64_t dw = smem_desc(w_src, 16, 1024), dx = smem_desc(w_src + W_TILE, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < TILE_K / 16; k++) umma_f16(tmem_base + buf * ACC_COLS, dw + (uint64_t)(2 * k), dx + (uint64_t)(2 * k), idesc, (i | k) != 0);
+                    umma_commit(smem_u32(&empty_bar[s]));
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
+                umma_commit(smem_u32(&tfull_bar[buf]));
+            }
+        }
+    } else if (warp >= FIRST_UNPACKER && warp < FIRST_EPILOGUE) {
+        // This thread: row `row` of the tile, half a slab's k (32 of 64): one 16-byte piece in, four out.
+        const int uw = warp - FIRST_UNPACKER, row = (uw & 3) * 32 + lane, half = uw >> 2, groups = (p.K - 1) / p.group + 1;
+        const uint32_t row_at = row * 128, turn = row & 7;
+        int s = 0, rs = 0;
+        uint32_t ph = 0, rph = 0;
+        for (int t = my_tile; t < p.tiles && ok; t += step) {
+            const int n = t % p.tiles_n * ROWS + row;
+            const T* scale_row = scales + (int64_t)(n < p.N ? n : 0) * groups;
+            const uint8_t* zero_row = ZEROS ? zeros + (int64_t)(n < p.N ? n : 0) * groups : nullptr;
+            const int k0 = first * SLAB_K + half * UNIT_K;
+            int which = k0 / p.group, in_group = k0 % p.group;
+            T scale = which < groups ? scale_row[which] : T(0.0f);   // past the end of K: X is zero there, and so is the scale
+            int zero = ZEROS && which < groups ? zero_row[which] : 8;
+            for (int i = 0; i < count; i++) {
+                uint32_t s2;
+                {
+                    const T both[2] = {scale, scale};
+                    s2 = *reinterpret_cast<const uint32_t*>(both);
+                }
+                const uint32_t z2 = zero_of(T(0.0f), zero);
+                for (in_group += TILE_K; in_group >= p.group; in_group -= p.group) which++;   // the next slab's scale, while this one waits
+                scale = which < groups ? scale_row[which] : T(0.0f);
+                if (ZEROS) zero = which < groups ? zero_row[which] : 8;
+                if (i % 4 == 0) {
+                    ok &= mbar_wait(smem_u32(&raw_full[rs]), rph, &gave_up);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                const uint4 w = load_shared_v4(raw + rs * RAW_BYTES + row_at + (((2 * (i % 4) + half) ^ turn) << 4));
+                if (i % 4 == 3 || i == count - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&raw_empty[rs]));
+                    if (++rs == p.raws) rs = 0, rph ^= 1;
+                }
+                const uint4 a = unpack_scaled<T>(w.x, z2, s2), b = unpack_scaled<T>(w.y, z2, s2), c = unpack_scaled<T>(w.z, z2, s2), d = unpack_scaled<T>(w.w, z2, s2);
+                ok &= mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t to = ring + s * stage_bytes + row_at;
+                store_shared_v4(to + (((4 * half + 0) ^ turn) << 4), a);
+                store_shared_v4(to + (((4 * half + 1) ^ turn) << 4), b);
+                store_shared_v4(to + (((4 * half + 2) ^ turn) << 4), c);
+                store_shared_v4(to + (((4 * half + 3) ^ turn) << 4), d);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads what this thread wrote
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&full_bar[s]));
+                if (++s == p.stages) s = 0, ph ^= 1;
+            }
+        }
+    } else if (warp >= FIRST_EPILOGUE && splits == 1) {
+        const int ew = warp & 3;   // this warp may touch lanes 32 ew .. 32 ew + 31
+        uint32_t local = 0;
+        for (int t = my_tile; t < p.tiles && ok; t += step, local++) {
+            const uint32_t buf = local & 1, use = local >> 1;
+            const int n = t % p.tiles_n * ROWS + ew * 32 + lane, m0 = t / p.tiles_n * p.tile_m, rows = min(p.tile_m, p.M - m0);
+            ok &= mbar_wait(smem_u32(&tfull_bar[buf]), use & 1, &gave_up);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t src = tmem_base + buf * ACC_COLS + ((uint32_t)(ew * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t r[16];
+                __syncwarp();
+                tmem_load_16(src + (uint32_t)c, r);
+                if (n < p.N) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (c + j < rows) store_as(C + (m0 + c + j) * ldc + n, __uint_as_float(r[j]));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[buf]));
+        }
+    }
+    __syncwarp();
+
+    if (splits > 1) {   // one tile a cluster: the CTAs' sums, added in the order of the CTAs
+        __syncthreads();   // the ring is done with: its memory takes the sums
+        float* sums = reinterpret_cast<float*>(smem_raw + (raw - smem_u32(smem_raw)));
+        const int n0 = my_tile % p.tiles_n * ROWS, m0 = my_tile / p.tiles_n * p.tile_m, rows = min(p.tile_m, p.M - m0);
+        if (warp >= FIRST_EPILOGUE) {
+            const int ew = warp & 3;
+            ok &= mbar_wait(smem_u32(&tfull_bar[0]), 0, &gave_up);   // on give-up the drain still runs on whatever tensor memory holds
+            ok = __all_sync(0xffffffffu, ok);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t r[16];
+                tmem_load_16(tmem_base + ((uint32_t)(ew * 32) << 16) + (uint32_t)c, r);
+#pragma unroll
+                for (int j = 0; j < 16; j++) sums[(c + j) * ROWS + ew * 32 + lane] = __uint_as_float(r[j]);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        for (int i = threadIdx.x; i < ((rows - split + splits - 1) / splits) * ROWS; i += TALL_THREADS) {
+            const int row = i % ROWS, c = i / ROWS * splits + split;
+            if (n0 + row >= p.N) continue;
+            const uint32_t at = smem_u32(&sums[c * ROWS + row]);
+            float v = 0.0f;
+            for (int q = 0; q < splits; q++) v += load_cluster_f32(map_to_cta(at, q));
+            store_as(C + (m0 + c) * ldc + n0 + row, v);
+        }
+        __syncwarp();
+        cluster_sync_all();   // no CTA leaves while another reads its sums
+    }
+    if (!ok && status) atomicExch(status, 1);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+}
+}  // namespace tall
+
 struct Args {
     const void *x, *w, *scales;
     const uint8_t* zeros;
@@ -308,8 +572,50 @@ int launch_flush(const Args& p) {
     return units % 4 == 0 ? launch_zeros<T, NT, 4>(p) : units % 2 == 0 ? launch_zeros<T, NT, 2>(p) : launch_zeros<T, NT, 1>(p);
 }
 
+template <class T, bool ZEROS>
+int launch_tall(const Args& p) {
+    const int sms = basalt_k::sm_count(), slabs = (p.K - 1) / SLAB_K + 1;
+    tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0};
+    // The width of a tile: of the few counts of tiles over M that come near 256 columns each, the one whose rounds over the SMs
+    // cost least. A slab costs two clocks a column, and not less than the unpacking of its weights, about 112 columns' worth.
+    int64_t best = INT64_MAX;
+    for (int tiles_m = (p.M - 1) / 256 + 1, tries = 0; tries < 4; tries++, tiles_m++) {
+        const int width = ((p.M - 1) / tiles_m + 16) / 16 * 16;
+        const int64_t tiles = (int64_t)((p.M - 1) / width + 1) * q.tiles_n, cost = ((tiles - 1) / sms + 1) * (width > 112 ? width : 112);
+        if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
+        if (cost < best) best = cost, q.tile_m = width, q.tiles = (int)tiles;
+    }
+    const int stage = tall::W_TILE + q.tile_m * tall::TILE_K * 2;
+    q.raws = q.tile_m > 192 ? 2 : tall::MAX_RAW;
+    q.stages = (tall::SMEM_MOST - 1024 - q.raws * tall::RAW_BYTES) / stage;
+    if (q.stages > tall::MAX_STAGES) q.stages = tall::MAX_STAGES;
+    const int smem = 1024 + q.raws * tall::RAW_BYTES + q.stages * stage;
+    int splits = 1;
+    while (splits < 8 && q.tiles * splits * 2 <= sms && slabs >= splits * 4) splits *= 2;
+    CUtensorMap mw, mx;
+    const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
+    if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, tall::TILE_K, q.tile_m)) return rc;
+    auto kern = tall::matmul_w4_tall<T, ZEROS>;
+    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, tall::SMEM_MOST)) return basalt_k::record(e, WHO);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits > 1 || q.tiles < sms ? q.tiles * splits : sms);
+    cfg.blockDim = dim3(tall::TALL_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = p.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return basalt_k::record(cudaLaunchKernelEx(&cfg, kern, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c, p.ldc, q, p.status), WHO);
+}
+
 template <class T>
-int launch_type(const Args& p) { return p.M <= 8 ? launch_flush<T, 1>(p) : p.M <= 16 ? launch_flush<T, 2>(p) : launch_flush<T, 4>(p); }
+int launch_type(const Args& p) {
+    if (p.M > 32 && p.N >= ROWS) return p.zeros ? launch_tall<T, true>(p) : launch_tall<T, false>(p);
+    return p.M <= 8 ? launch_flush<T, 1>(p) : p.M <= 16 ? launch_flush<T, 2>(p) : launch_flush<T, 4>(p);
+}
 
 }  // namespace
 
