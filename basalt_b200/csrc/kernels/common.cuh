@@ -4,6 +4,7 @@
 
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 
 namespace basalt_k {
@@ -28,6 +29,37 @@ inline bool overlap(const Span& a, const Span& b) {
     if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
     const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
     return a0 < b0 + (uintptr_t)(((b.rows - 1) * b.ld + b.cols) * b.size) && b0 < a0 + (uintptr_t)(((a.rows - 1) * a.ld + a.cols) * a.size);
+}
+
+// Lets KERNEL have `bytes` of dynamic shared memory on the current device; asked of the runtime once a kernel and device.
+template <auto KERNEL>
+int allow_smem(const char* who, int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device)) return record(e, who);
+    if (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1)) return 0;
+    if (const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return record(e, who);
+    if (device < 64) done.fetch_or((uint64_t)1 << device, std::memory_order_relaxed);
+    return 0;
+}
+
+// Launches `kernel` on `grid` CTAs in clusters of `cluster`, with programmatic stream serialisation: its prologue may run
+// while the kernel before it in the stream drains, so it has to call tc::wait_for_predecessor() before it touches global memory.
+template <class... P, class... A>
+int launch_clusters(const char* who, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return record(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), who);
 }
 
 // Resident CTAs per SM for `kernel` at the given block size, from the occupancy calculator.

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
 
     if (threadIdx.x == 0) {
-        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;   // an earlier CTA gave up: do not pile on
+        gave_up = 0;
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
@@ -86,6 +86,8 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_acc = tmem_slot;
+    wait_for_predecessor();
+    if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
 
     if (warp == 0 && lane == 0) {
@@ -183,7 +185,7 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* m,
 
 // VECTORS: C's rows are whole 16-byte pieces from an aligned start.
 template <class T, bool VECTORS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
     matmul_e4m3_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const float* __restrict__ a_scales,
                      const float* __restrict__ b_scales, T* __restrict__ C, int64_t ldc, int M, int N, int K, int32_t* status) {
     extern __shared__ uint8_t smem_raw[];
@@ -198,7 +200,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     const int tiles_m = (M - 1) / TM + 1, tiles_n = (N - 1) / TN + 1, num_tiles = tiles_m * tiles_n, slabs = (K - 1) / BK + 1;
 
     if (threadIdx.x == 0) {
-        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;
+        gave_up = 0;
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);    // the leader's producer; bytes arrive from both CTAs
             mbar_init(smem_u32(&empty_bar[s]), 1);   // one commit of the leader's MMA warp
@@ -219,6 +221,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     cluster_sync_all();   // the peer's barriers are initialised before anything can signal them
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
+    wait_for_predecessor();
+    if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
 
     if (warp == 0) {
@@ -357,25 +361,16 @@ int launch(const Args& p) {
     CUtensorMap ma, mb;
     if (const int rc = make_tensor_map(&mb, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.b, p.N, p.K, p.ldb, BK, BN)) return rc;
     if (const int rc = make_tensor_map(&ma, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, p.M, p.K, p.lda, BK, TN)) return rc;
-    auto kern = matmul_e4m3_kernel<T, TN>;
+    constexpr auto kern = matmul_e4m3_kernel<T, TN>;
     constexpr int smem = smem_of<TN>();
-    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return basalt_k::record(e, WHO);
+    if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
     const int tiles_n = (p.N - 1) / BN + 1, slabs = (p.K - 1) / BK + 1;
     const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TN + 1);
     int splits = 1;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps four slabs
     while (splits < 8 && tiles * splits * 2 <= 2 * basalt_k::sm_count() && slabs >= splits * 8) splits *= 2;
     if (tiles * splits > INT32_MAX) return basalt_k::record_msg(1, WHO, "M * N is too large");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = p.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return basalt_k::record(cudaLaunchKernelEx(&cfg, kern, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, tiles_n, p.status), WHO);
+    return basalt_k::launch_clusters(WHO, kern, (unsigned)(tiles * splits), THREADS, smem, splits, p.stream, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K,
+                                     tiles_n, p.status);
 }
 
 template <class T, bool VECTORS>
@@ -383,13 +378,12 @@ int launch_pair(const Args& p) {
     CUtensorMap ma, mb;
     if (const int rc = make_tensor_map(&ma, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, p.M, p.K, p.lda, BK, pair::HALF)) return rc;
     if (const int rc = make_tensor_map(&mb, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.b, p.N, p.K, p.ldb, BK, pair::HALF)) return rc;
-    auto kern = pair::matmul_e4m3_pair<T, VECTORS>;
-    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM)) return basalt_k::record(e, WHO);
+    constexpr auto kern = pair::matmul_e4m3_pair<T, VECTORS>;
+    if (const int rc = basalt_k::allow_smem<kern>(WHO, pair::SMEM)) return rc;
     const int64_t tiles = (int64_t)((p.M - 1) / pair::TM + 1) * ((p.N - 1) / pair::TN + 1);
     if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
     const int pairs = (int)(tiles < basalt_k::sm_count() / 2 ? tiles : basalt_k::sm_count() / 2);
-    kern<<<2 * pairs, pair::PAIR_THREADS, pair::SMEM, p.stream>>>(ma, mb, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, p.status);
-    return basalt_k::record(cudaGetLastError(), WHO);
+    return basalt_k::launch_clusters(WHO, kern, 2 * pairs, pair::PAIR_THREADS, pair::SMEM, 2, p.stream, ma, mb, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, p.status);
 }
 
 template <class T>

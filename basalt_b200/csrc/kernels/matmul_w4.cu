@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
 
     if (threadIdx.x == 0) {
-        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;
+        gave_up = 0;
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), CONSUMERS);
@@ -142,6 +142,8 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
+    wait_for_predecessor();
+    if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
     float total[2][NT][4] = {};
 
@@ -169,28 +171,47 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
         const int groups = (K - 1) / group + 1;
         const T* scale_row[4];
         const uint8_t* zero_row[4];
-        bool row_in[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int n = n0 + row0 + g + 8 * r;
-            row_in[r] = n < N;
-            scale_row[r] = scales + (int64_t)(row_in[r] ? n : 0) * groups;
-            zero_row[r] = ZEROS ? zeros + (int64_t)(row_in[r] ? n : 0) * groups : nullptr;
+            const int64_t n = min(n0 + row0 + g + 8 * r, N - 1);   // rows past the last are computed with its scales, and not stored
+            scale_row[r] = scales + n * groups;
+            zero_row[r] = ZEROS ? zeros + n * groups : nullptr;
         }
-        for (int i = 0; i < count; i++) {
-            const int s = i % STAGES;
-            float scale[4 / FLUSH][4];
-            int zero[4 / FLUSH][4];
+        // The scales of a slab are loaded while the slab before is computed.
+        T scale[4 / FLUSH][4];
+        uint8_t zero[4 / FLUSH][4];
+        int which[4 / FLUSH], in_group[4 / FLUSH];
+        auto load_scales = [&]() {
 #pragma unroll
             for (int f = 0; f < 4 / FLUSH; f++) {
-                const int which = ((first + i) * SLAB_K + half * 128 + f * FLUSH * UNIT_K) / group;
-                const bool in = which < groups;   // past the end of K: X is zero there, and so is the scale
+                const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    scale[f][r] = in && row_in[r] ? to_float(scale_row[r][which]) : 0.0f;
-                    zero[f][r] = ZEROS && in ? zero_row[r][which] : 8;
+                    scale[f][r] = in ? scale_row[r][which[f]] : T(0.0f);
+                    if (ZEROS) zero[f][r] = in ? zero_row[r][which[f]] : 0;
                 }
+                for (in_group[f] += SLAB_K; in_group[f] >= group; in_group[f] -= group) which[f]++;
             }
+        };
+#pragma unroll
+        for (int f = 0; f < 4 / FLUSH; f++) {
+            const int k = first * SLAB_K + half * 128 + f * FLUSH * UNIT_K;
+            which[f] = k / group, in_group[f] = k % group;
+        }
+        load_scales();
+        for (int i = 0; i < count; i++) {
+            const int s = i % STAGES;
+            float by[4 / FLUSH][4];
+            Zero<T> z[ZEROS ? 4 / FLUSH : 1][ZEROS ? 4 : 1];
+            if (!ZEROS) z[0][0].set(8);
+#pragma unroll
+            for (int f = 0; f < 4 / FLUSH; f++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    by[f][r] = to_float(scale[f][r]);
+                    if (ZEROS) z[f][r].set(zero[f][r]);
+                }
+            load_scales();
             ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -199,15 +220,12 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 #pragma unroll
             for (int f = 0; f < 4 / FLUSH; f++) {
                 float acc[2][NT][4] = {};
-                Zero<T> z[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) z[r].set(zero[f][r]);
 #pragma unroll
                 for (int v = 0; v < FLUSH; v++) {
                     const int u = f * FLUSH + v;
                     uint32_t a[4][4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) unpack(load_shared_u32(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), z[r], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
+                    for (int r = 0; r < 4; r++) unpack(load_shared_u32(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), z[ZEROS ? f : 0][ZEROS ? r : 0], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         const uint4 x = load_shared_v4(x_at + u * TOKENS * X_BOX_K * 2 + nt * 8 * X_BOX_K * 2);   // row 8 nt + g of X, its k 8 t .. 8 t + 7 of the unit
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) total[h][nt][j] += scale[f][2 * h + (j >> 1)] * acc[h][nt][j];
+                        for (int j = 0; j < 4; j++) total[h][nt][j] += by[f][2 * h + (j >> 1)] * acc[h][nt][j];
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
@@ -316,7 +334,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     const int x_bytes = p.tile_m * TILE_K * 2, stage_bytes = W_TILE + x_bytes;
 
     if (threadIdx.x == 0) {
-        gave_up = status && *reinterpret_cast<volatile int32_t*>(status) != 0;
+        gave_up = 0;
         for (int s = 0; s < p.stages; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1 + UNPACKERS);   // the rows of X, and each unpacking warp
             mbar_init(smem_u32(&empty_bar[s]), 1);
@@ -340,6 +358,8 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
+    wait_for_predecessor();
+    if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
 
     if (warp == WARP_X) {
@@ -541,26 +561,16 @@ int launch(const Args& p) {
     const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
     if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, X_BOX_K, 8 * NT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
-    auto kern = matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
+    constexpr auto kern = matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
     constexpr int smem = smem_of<NT>();
-    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return basalt_k::record(e, WHO);
+    if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
     const int tiles_n = (p.N - 1) / ROWS + 1, slabs = (p.K - 1) / SLAB_K + 1;
     const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / (8 * NT) + 1);
     int splits = 1;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps two slabs
     while (splits < 8 && tiles * splits * 2 <= 2 * basalt_k::sm_count() && slabs >= splits * 4) splits *= 2;
     if (tiles * splits > INT32_MAX) return basalt_k::record_msg(1, WHO, "M * N is too large");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = p.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return basalt_k::record(
-        cudaLaunchKernelEx(&cfg, kern, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c, p.ldc, p.M, p.N, p.K, p.group, tiles_n, p.status), WHO);
+    return basalt_k::launch_clusters(WHO, kern, (unsigned)(tiles * splits), THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c, p.ldc, p.M, p.N, p.K,
+                                     p.group, tiles_n, p.status);
 }
 
 template <class T, int NT, int FLUSH>
@@ -596,19 +606,10 @@ int launch_tall(const Args& p) {
     const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
     if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, tall::TILE_K, q.tile_m)) return rc;
-    auto kern = tall::matmul_w4_tall<T, ZEROS>;
-    if (const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, tall::SMEM_MOST)) return basalt_k::record(e, WHO);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits > 1 || q.tiles < sms ? q.tiles * splits : sms);
-    cfg.blockDim = dim3(tall::TALL_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = p.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return basalt_k::record(cudaLaunchKernelEx(&cfg, kern, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c, p.ldc, q, p.status), WHO);
+    constexpr auto kern = tall::matmul_w4_tall<T, ZEROS>;
+    if (const int rc = basalt_k::allow_smem<kern>(WHO, tall::SMEM_MOST)) return rc;
+    return basalt_k::launch_clusters(WHO, kern, splits > 1 || q.tiles < sms ? q.tiles * splits : sms, tall::TALL_THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales,
+                                     p.zeros, (T*)p.c, p.ldc, q, p.status);
 }
 
 template <class T>

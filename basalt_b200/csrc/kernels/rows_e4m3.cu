@@ -19,6 +19,7 @@
 
 #include "../../../include/basalt_b200_kernels.h"
 #include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace {
 
@@ -31,7 +32,7 @@ struct Rows {
     float* scales;
     int64_t ldx, ldr, ldt, ldy;
     int rows, cols;
-    float eps;
+    float eps, per_col;   // per_col: 1 / cols
 };
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -119,21 +120,26 @@ __device__ __forceinline__ void join_row(float& sum, float& top) {
     }
 }
 
-// What the row's outputs are multiplied by, from the joined numbers; the row's first thread stores the scale.
+// What the row's outputs are multiplied by, from the joined numbers; the row's first thread stores the scale. The reciprocal
+// square root and the reciprocal are the hardware's (each off by at most two f32 steps, 2^-22 of the value): the exact ones cost every thread
+// more instructions than its elements do.
 template <bool NORM, bool E4M3>
 __device__ __forceinline__ float row_factor(const Rows& p, int row, bool active, float sum, float top) {
-    const float r = NORM ? 1.0f / sqrtf(sum / (float)p.cols + p.eps) : 1.0f;
+    const float r = NORM ? rsqrtf(sum * p.per_col + p.eps) : 1.0f;
     if (!E4M3) return r;
-    float scale = top * r / E4M3_MAX;
-    if (scale < SCALE_MIN) scale = SCALE_MIN;   // false for a NaN, which stays
-    if (active && threadIdx.x == 0) p.scales[row] = scale;
-    return r * (1.0f / scale);   // off by two more f32 roundings than y / s, 2^-20 of an e4m3 step
+    float most = top * r;
+    if (most < E4M3_MAX * SCALE_MIN) most = E4M3_MAX * SCALE_MIN;   // false for a NaN, which stays
+    if (active && threadIdx.x == 0) p.scales[row] = most / E4M3_MAX;
+    float inverse;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(most));
+    return r * (E4M3_MAX * inverse);
 }
 
 // Rows whose pointers, strides and width are whole 16-byte vectors, V of them in each thread's registers.
 template <class T, bool NORM, bool E4M3, int V>
 __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const Rows p) {
     constexpr int W = VEC<T>;
+    basalt_k::tc::wait_for_predecessor();
     const int64_t row64 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const bool active = row64 < p.rows;
     const int row = active ? (int)row64 : 0, vectors = active ? p.cols / W : 0;
@@ -193,6 +199,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
 // from cache). Only the second pass writes, so that total may be the residual's own buffer.
 template <class T, bool NORM, bool E4M3>
 __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
+    basalt_k::tc::wait_for_predecessor();
     const int row = blockIdx.x;
     const T* x = (const T*)p.x + row * p.ldx;
     const T* residual = NORM && p.residual ? (const T*)p.residual + row * p.ldr : nullptr;
@@ -230,10 +237,12 @@ int launch(const Rows& p, const char* who, cudaStream_t s) {
     const bool y_vec = eight ? (uintptr_t)p.y % W == 0 && p.ldy % W == 0 : (uintptr_t)p.y % 16 == 0 && p.ldy % W == 0;
     const int64_t vectors = p.cols / W;
     if (all % 16 || strides % W || !y_vec || vectors > 8 * 512) {
-        rows_twice<T, NORM, E4M3><<<p.rows, 512, 0, s>>>(p);
-        return basalt_k::record(cudaGetLastError(), who);
+        return basalt_k::launch_clusters(who, rows_twice<T, NORM, E4M3>, p.rows, 512, 0, 1, s, p);
     }
-    const int v = vectors <= 1024 ? 1 : vectors <= 4 * 512 ? 4 : 8;
+    // Vectors a thread: one where the rows are few and each should be over soon; four where there are rows for every SM, so that
+    // what a thread spends on joining and on the row's factor is shared by more elements.
+    const bool few = p.rows <= basalt_k::sm_count();
+    const int v = vectors <= 1024 && few ? 1 : vectors <= 4 * 512 ? 4 : 8;
     int tpr = (int)((vectors + v - 1) / v);
     if (tpr > 32) tpr = (tpr + 31) / 32 * 32;
     else {
@@ -243,10 +252,8 @@ int launch(const Rows& p, const char* who, cudaStream_t s) {
     }
     const int per_block = tpr >= 128 ? 1 : 128 / tpr;
     const dim3 block(tpr, per_block), grid((unsigned)(((int64_t)p.rows + per_block - 1) / per_block));
-    if (v == 1) rows_in_registers<T, NORM, E4M3, 1><<<grid, block, 0, s>>>(p);
-    else if (v == 4) rows_in_registers<T, NORM, E4M3, 4><<<grid, block, 0, s>>>(p);
-    else rows_in_registers<T, NORM, E4M3, 8><<<grid, block, 0, s>>>(p);
-    return basalt_k::record(cudaGetLastError(), who);
+    auto kern = v == 1 ? rows_in_registers<T, NORM, E4M3, 1> : v == 2 ? rows_in_registers<T, NORM, E4M3, 2> : v == 4 ? rows_in_registers<T, NORM, E4M3, 4> : rows_in_registers<T, NORM, E4M3, 8>;
+    return basalt_k::launch_clusters(who, kern, grid, block, 0, 1, s, p);
 }
 
 template <bool NORM, bool E4M3>
@@ -295,7 +302,7 @@ extern "C" int basalt_k_rms_norm(int type, const void* x, int64_t ldx, const voi
     if (!(eps >= 0.0f)) return basalt_k::record_msg(1, who, "eps must not be negative");
     if (rows == 0) return 0;
     if (const int rc = basalt_k::check_device_pointers(who, {x, residual, total, weight, y, scales})) return rc;
-    const Rows p = {x, residual, weight, total, y, scales, ldx, ldr, ldt, ldy, (int)rows, (int)cols, eps};
+    const Rows p = {x, residual, weight, total, y, scales, ldx, ldr, ldt, ldy, (int)rows, (int)cols, eps, 1.0f / (float)cols};
     return scales ? launch_type<true, true>(type, p, who, (cudaStream_t)stream) : launch_type<true, false>(type, p, who, (cudaStream_t)stream);
 }
 
@@ -305,6 +312,6 @@ extern "C" int basalt_k_quantize_e4m3(int type, const void* x, int64_t ldx, void
     if (const int rc = check_rows(who, type, rows, cols, {x, rows, cols, ldx, type == BASALT_K_TYPE_F32 ? 4 : 2}, {}, {}, {q, rows, cols, ldq, 1}, scales, nullptr)) return rc;
     if (rows == 0) return 0;
     if (const int rc = basalt_k::check_device_pointers(who, {x, q, scales})) return rc;
-    const Rows p = {x, nullptr, nullptr, nullptr, q, scales, ldx, 0, 0, ldq, (int)rows, (int)cols, 0.0f};
+    const Rows p = {x, nullptr, nullptr, nullptr, q, scales, ldx, 0, 0, ldq, (int)rows, (int)cols, 0.0f, 0.0f};
     return launch_type<false, true>(type, p, who, (cudaStream_t)stream);
 }

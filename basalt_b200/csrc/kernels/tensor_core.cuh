@@ -105,6 +105,13 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// For kernels launched by launch_clusters or launch_rows: lets the kernel behind this one begin its prologue, and waits until
+// the one before has finished and its results can be seen. Everything up to here touches no global memory.
+__device__ __forceinline__ void wait_for_predecessor() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---- clusters and CTA pairs ----
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
