@@ -38,9 +38,12 @@ struct Rows {
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ float load_one(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_one(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <class T>
+__device__ __forceinline__ T rounded(float v) {
+    if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+    else return v;
+}
 
 template <class T>
 constexpr int VEC = 16 / sizeof(T);
@@ -60,8 +63,7 @@ __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
     }
 }
 template <class T>
-__device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC<T>]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void values(const uint4& u, float (&f)[VEC<T>]) {
     if constexpr (sizeof(T) == 4) unpack(u, f);
     else unpack<T>(u, f);
 }
@@ -135,68 +137,158 @@ __device__ __forceinline__ float row_factor(const Rows& p, int row, bool active,
     return r * (E4M3_MAX * inverse);
 }
 
-// Rows whose pointers, strides and width are whole 16-byte vectors, V of them in each thread's registers.
-template <class T, bool NORM, bool E4M3, int V>
+// The largest magnitude in a vector of T; 16-bit values are compared two at a time as they are.
+template <class T>
+__device__ __forceinline__ float magnitude(const uint4& u) {
+    if constexpr (sizeof(T) == 4) {
+        return max_nan(max_nan(fabsf(__uint_as_float(u.x)), fabsf(__uint_as_float(u.y))), max_nan(fabsf(__uint_as_float(u.z)), fabsf(__uint_as_float(u.w))));
+    } else {
+        using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+        const uint32_t w[4] = {u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu, u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu};
+        const T2* v = reinterpret_cast<const T2*>(w);
+        const T2 m = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+        return max_nan(load_one(&m.x), load_one(&m.y));
+    }
+}
+
+// Rows whose pointers, strides and width are whole 16-byte vectors, V of them in each thread's registers. Every load of the
+// row is issued before its first use and before any store (an output may be an input's buffer, so the compiler
+// keeps their order): the loads in flight are what the memory is kept busy with. Without a residual the row stays
+// in its own type until it is written; with one, h is kept in f32.
+template <class T, bool NORM, bool RESIDUAL, bool E4M3, int V>
 __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const Rows p) {
     constexpr int W = VEC<T>;
     basalt_k::tc::wait_for_predecessor();
     const int64_t row64 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const bool active = row64 < p.rows;
     const int row = active ? (int)row64 : 0, vectors = active ? p.cols / W : 0;
-    const T* x = (const T*)p.x + row * p.ldx;
-    float h[V][W], sum = 0.0f, top = 0.0f;
+    const uint4* x = (const uint4*)((const T*)p.x + row * p.ldx) + threadIdx.x;
+    uint4 raw[V];
 #pragma unroll
-    for (int v = 0; v < V; v++) {
-        const int i = threadIdx.x + v * blockDim.x;
-        if (i < vectors) load_vec(x + (int64_t)i * W, h[v]);
-    }
-    if (NORM && p.residual) {
-        const T* residual = (const T*)p.residual + row * p.ldr;
+    for (int v = 0; v < V; v++)
+        if (threadIdx.x + v * blockDim.x < vectors) raw[v] = x[v * blockDim.x];
+    float h[RESIDUAL ? V : 1][W], sum = 0.0f, top = 0.0f;
+    if constexpr (RESIDUAL) {
+        const uint4* residual = (const uint4*)((const T*)p.residual + row * p.ldr) + threadIdx.x;
+        uint4 more[V];
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (threadIdx.x + v * blockDim.x < vectors) more[v] = residual[v * blockDim.x];
+        T* total = (T*)p.total + row * p.ldt + threadIdx.x * W;
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            const int i = threadIdx.x + v * blockDim.x;
-            if (i >= vectors) continue;
+            if (threadIdx.x + v * blockDim.x >= vectors) continue;
             float r[W];
-            load_vec(residual + (int64_t)i * W, r);
+            values<T>(raw[v], h[v]);
+            values<T>(more[v], r);
 #pragma unroll
             for (int j = 0; j < W; j++) h[v][j] += r[j];
-            if (p.total) store_vec((T*)p.total + row * p.ldt + (int64_t)i * W, h[v]);
+            if (p.total) store_vec(total + v * blockDim.x * W, h[v]);
         }
     }
+    const uint4* weight = (const uint4*)p.weight + threadIdx.x;
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const int i = threadIdx.x + v * blockDim.x;
-        if (i >= vectors) continue;
-        if (NORM) {
+        if (threadIdx.x + v * blockDim.x >= vectors) continue;
+        if constexpr (!NORM) top = max_nan(top, magnitude<T>(raw[v]));
+        else {
+            float once[W];
+            float(&e)[W] = RESIDUAL ? h[v] : once;
+            if (!RESIDUAL) values<T>(raw[v], e);
 #pragma unroll
-            for (int j = 0; j < W; j++) sum += h[v][j] * h[v][j];
-            if (p.weight) {
+            for (int j = 0; j < W; j++) sum += e[j] * e[j];
+            if (p.weight && (E4M3 || RESIDUAL)) {
                 float w[W];
-                load_vec((const T*)p.weight + (int64_t)i * W, w);
+                values<T>(weight[v * blockDim.x], w);
 #pragma unroll
-                for (int j = 0; j < W; j++) h[v][j] *= w[j];
+                for (int j = 0; j < W; j++) e[j] *= w[j];
             }
-        }
-        if (E4M3) {
+            if (E4M3) {
 #pragma unroll
-            for (int j = 0; j < W; j++) top = max_nan(top, fabsf(h[v][j]));
+                for (int j = 0; j < W; j++) top = max_nan(top, fabsf(e[j]));
+            }
         }
     }
     join_row(sum, top);
     const float f = row_factor<NORM, E4M3>(p, row, active, sum, top);
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const int i = threadIdx.x + v * blockDim.x;
-        if (i >= vectors) continue;
+        if (threadIdx.x + v * blockDim.x >= vectors) continue;
+        float once[W];
+        float(&e)[W] = RESIDUAL ? h[v] : once;
+        if (!RESIDUAL) {
+            values<T>(raw[v], e);
+            if (NORM && p.weight) {
+                float w[W];
+                values<T>(weight[v * blockDim.x], w);
 #pragma unroll
-        for (int j = 0; j < W; j++) h[v][j] *= f;
-        if constexpr (E4M3) store_e4m3((uint8_t*)p.y + row * p.ldy + (int64_t)i * W, h[v]);
-        else store_vec((T*)p.y + row * p.ldy + (int64_t)i * W, h[v]);
+                for (int j = 0; j < W; j++) e[j] *= w[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < W; j++) e[j] *= f;
+        const int at = (threadIdx.x + v * blockDim.x) * W;
+        if constexpr (E4M3) store_e4m3((uint8_t*)p.y + row * p.ldy + at, e);
+        else store_vec((T*)p.y + row * p.ldy + at, e);
     }
 }
 
-// Any alignment, any width: a block per row, element by element, the row read twice (the second time
-// from cache). Only the second pass writes, so that total may be the residual's own buffer.
+// Rows that start at no vector boundary, or whose width is no whole number of vectors, up to EACH * 512 elements: a block per
+// row, element by element, one read of the row.
+constexpr int EACH = 16;
+template <class T, bool NORM, bool RESIDUAL, bool E4M3>
+__global__ void __launch_bounds__(512) rows_by_element(const Rows p) {
+    basalt_k::tc::wait_for_predecessor();
+    const int row = blockIdx.x;
+    const T* x = (const T*)p.x + row * p.ldx + threadIdx.x;
+    const int left = p.cols - threadIdx.x, step = blockDim.x;   // element v of this thread is in the row where v * step < left
+    T raw[EACH], more[RESIDUAL ? EACH : 1];
+#pragma unroll
+    for (int v = 0; v < EACH; v++)
+        if (v * step < left) raw[v] = x[v * step];
+    if constexpr (RESIDUAL) {
+        const T* residual = (const T*)p.residual + row * p.ldr + threadIdx.x;
+#pragma unroll
+        for (int v = 0; v < EACH; v++)
+            if (v * step < left) more[v] = residual[v * step];
+    }
+    T by[NORM ? EACH : 1];
+    const bool weighted = NORM && p.weight;
+    if constexpr (NORM) {
+        const T* weight = (const T*)p.weight + threadIdx.x;
+#pragma unroll
+        for (int v = 0; v < EACH; v++)
+            if (weighted && v * step < left) by[v] = weight[v * step];
+    }
+    T* total = RESIDUAL && p.total ? (T*)p.total + row * p.ldt + threadIdx.x : nullptr;
+    float h[EACH], sum = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int v = 0; v < EACH; v++) {
+        const bool in = v * step < left;
+        h[v] = in ? load_one(&raw[v]) : 0.0f;
+        if constexpr (RESIDUAL) {
+            if (in) h[v] += load_one(&more[v]);
+            if (in && total) total[v * step] = rounded<T>(h[v]);
+        }
+        sum += h[v] * h[v];
+        if constexpr (NORM)
+            if (in && weighted) h[v] *= load_one(&by[v]);
+        if (E4M3) top = max_nan(top, fabsf(h[v]));
+    }
+    join_row(sum, top);
+    const float f = row_factor<NORM, E4M3>(p, row, true, sum, top);
+    T* y = (T*)p.y + row * p.ldy + threadIdx.x;
+    uint8_t* bytes = (uint8_t*)p.y + row * p.ldy + threadIdx.x;
+#pragma unroll
+    for (int v = 0; v < EACH; v++) {
+        if (v * step >= left) continue;
+        if constexpr (E4M3) bytes[v * step] = (uint8_t)__nv_cvt_float_to_fp8(h[v] * f, __NV_SATFINITE, __NV_E4M3);
+        else y[v * step] = rounded<T>(h[v] * f);
+    }
+}
+
+// Any alignment, any width: a block per row, element by element, the row read twice (the second time from
+// cache). Only the second pass writes, so that total may be the residual's own buffer.
 template <class T, bool NORM, bool E4M3>
 __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
     basalt_k::tc::wait_for_predecessor();
@@ -218,11 +310,11 @@ __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
         float h = load_one(x + i);
         if (residual) {
             h += load_one(residual + i);
-            if (p.total) store_one((T*)p.total + row * p.ldt + i, h);
+            if (p.total) ((T*)p.total)[row * p.ldt + i] = rounded<T>(h);
         }
         if (weight) h *= load_one(weight + i);
         if (E4M3) ((uint8_t*)p.y)[row * p.ldy + i] = (uint8_t)__nv_cvt_float_to_fp8(h * f, __NV_SATFINITE, __NV_E4M3);
-        else store_one((T*)p.y + row * p.ldy + i, h * f);
+        else ((T*)p.y)[row * p.ldy + i] = rounded<T>(h * f);
     }
 }
 
@@ -236,7 +328,16 @@ int launch(const Rows& p, const char* who, cudaStream_t s) {
     if (p.total) strides |= p.ldt;
     const bool y_vec = eight ? (uintptr_t)p.y % W == 0 && p.ldy % W == 0 : (uintptr_t)p.y % 16 == 0 && p.ldy % W == 0;
     const int64_t vectors = p.cols / W;
-    if (all % 16 || strides % W || !y_vec || vectors > 8 * 512) {
+    const bool by_vector = all % 16 == 0 && strides % W == 0 && y_vec;
+    if (!by_vector && p.cols <= EACH * 512) {
+        auto kern = rows_by_element<T, NORM, false, E4M3>;
+        if constexpr (NORM)
+            if (p.residual) kern = rows_by_element<T, NORM, true, E4M3>;
+        // every slot of a thread is worked through, used or not: as few threads as hold a long row, more for a short one
+        const int each = p.cols > 4 * 256 ? EACH : 4, threads = ((p.cols + each - 1) / each + 31) / 32 * 32;
+        return basalt_k::launch_clusters(who, kern, p.rows, threads, 0, 1, s, p);
+    }
+    if (!by_vector || vectors > 8 * 512) {
         return basalt_k::launch_clusters(who, rows_twice<T, NORM, E4M3>, p.rows, 512, 0, 1, s, p);
     }
     // Vectors a thread: one where the rows are few and each should be over soon; four where there are rows for every SM, so that
@@ -252,7 +353,13 @@ int launch(const Rows& p, const char* who, cudaStream_t s) {
     }
     const int per_block = tpr >= 128 ? 1 : 128 / tpr;
     const dim3 block(tpr, per_block), grid((unsigned)(((int64_t)p.rows + per_block - 1) / per_block));
-    auto kern = v == 1 ? rows_in_registers<T, NORM, E4M3, 1> : v == 2 ? rows_in_registers<T, NORM, E4M3, 2> : v == 4 ? rows_in_registers<T, NORM, E4M3, 4> : rows_in_registers<T, NORM, E4M3, 8>;
+    const auto pick = [&](auto residual) {
+        constexpr bool R = decltype(residual)::value;
+        return v == 1 ? rows_in_registers<T, NORM, R, E4M3, 1> : v == 4 ? rows_in_registers<T, NORM, R, E4M3, 4> : rows_in_registers<T, NORM, R, E4M3, 8>;
+    };
+    auto kern = pick(std::false_type());
+    if constexpr (NORM)
+        if (p.residual) kern = pick(std::true_type());
     return basalt_k::launch_clusters(who, kern, grid, block, 0, 1, s, p);
 }
 
