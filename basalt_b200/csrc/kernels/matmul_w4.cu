@@ -36,23 +36,12 @@ constexpr int UNIT_K = 32, X_BOX_K = 32;   // a unit: the 32 k that one 16-byte 
 template <int NT>
 __host__ __device__ constexpr int x_bytes_of() { return 8 * NT * SLAB_K * 2; }
 template <int NT>
-__host__ __device__ constexpr int stages_of() { return NT == 1 ? 5 : NT == 2 ? 4 : 3; }   // at most 100 KB: two CTAs fit an SM
+__host__ __device__ constexpr int stages_of() { return NT == 1 ? 5 : 3; }
 template <int NT>
-__host__ __device__ constexpr int smem_of() { return stages_of<NT>() * (W_BYTES + x_bytes_of<NT>()) + 1024; }
+__host__ __device__ constexpr int join_bytes_of() { return 2 * 8 * NT * ROWS * 4; }   // the sums of both halves of the warps, for every row of X
+template <int NT>
+__host__ __device__ constexpr int smem_of() { return stages_of<NT>() * (W_BYTES + x_bytes_of<NT>()) + join_bytes_of<NT>() + 1024; }   // at most 113 KB: two CTAs fit an SM
 
-__device__ __forceinline__ uint32_t load_shared_u32(uint32_t at) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ uint4 load_shared_v4(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
-}
-__device__ __forceinline__ void store_shared_v4(uint32_t at, const uint4& v) {
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
@@ -73,13 +62,24 @@ struct Zero<__half> {
     __half2 low, high;
     __device__ __forceinline__ void set(int z) {
         low = __half2half2(__int2half_rn(1024 + z));
-        high = __half2half2(__int2half_rn(-64 - z));
+        high = __hsub2(__half2half2(__int2half_rn(960)), low);   // -64 - z
+    }
+    __device__ __forceinline__ Zero of_lane(int lane) const {
+        Zero v;
+        v.low = __shfl_sync(0xffffffffu, low, lane);
+        v.high = __hsub2(__half2half2(__int2half_rn(960)), v.low);
+        return v;
     }
 };
 template <>
 struct Zero<__nv_bfloat16> {
     __nv_bfloat162 low;
     __device__ __forceinline__ void set(int z) { low = __bfloat162bfloat162(__int2bfloat16_rn(128 + z)); }
+    __device__ __forceinline__ Zero of_lane(int lane) const {
+        Zero v;
+        v.low = __shfl_sync(0xffffffffu, low, lane);
+        return v;
+    }
 };
 
 // Eight packed weights -> q - z as pairs of k: (0, 4), (1, 5), (2, 6), (3, 7). The four bits are put into the mantissa of a
@@ -107,11 +107,11 @@ __device__ __forceinline__ void unpack(uint32_t w, const Zero<__nv_bfloat16>& z,
 template <class T>
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same_v<T, __half>)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
     __shared__ volatile uint32_t gave_up;
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (ring - smem_u32(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
     const int tile = blockIdx.x / splits, n0 = tile % tiles_n * ROWS, m0 = tile / tiles_n * TOKENS;
@@ -133,6 +134,8 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
 
     if (threadIdx.x == 0) {
+        prefetch_map(&map_w);
+        prefetch_map(&map_x);
         gave_up = 0;
         for (int s = 0; s < STAGES; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
@@ -142,6 +145,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
+    cluster_arrive();
     wait_for_predecessor();
     if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
@@ -155,7 +159,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
                 if (!ok) break;
                 const uint32_t fb = smem_u32(&full_bar[s]), w_dst = ring + s * STAGE_BYTES, x_dst = w_dst + W_BYTES;
                 const int k = (first + i) * SLAB_K;
-                mbar_expect_tx(fb, STAGE_BYTES);
+                mbar_expect_tx(fb, W_BYTES + min(M, TOKENS) * SLAB_K * 2);
                 tma_load_2d(w_dst, &map_w, fb, k / 2, n0);
 #pragma unroll
                 for (int b = 0; b < SLAB_K / X_BOX_K; b++) tma_load_2d(x_dst + b * TOKENS * X_BOX_K * 2, &map_x, fb, k + b * X_BOX_K, m0);
@@ -169,27 +173,20 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     } else {
         const int half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
         const int groups = (K - 1) / group + 1;
-        const T* scale_row[4];
-        const uint8_t* zero_row[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int64_t n = min(n0 + row0 + g + 8 * r, N - 1);   // rows past the last are computed with its scales, and not stored
-            scale_row[r] = scales + n * groups;
-            zero_row[r] = ZEROS ? zeros + n * groups : nullptr;
-        }
-        // The scales of a slab are loaded while the slab before is computed.
-        T scale[4 / FLUSH][4];
-        uint8_t zero[4 / FLUSH][4];
+        // Of the four weight rows g, g + 8, g + 16 and g + 24 that four lanes share, lane t loads the scales of row g + 8 t and the
+        // lanes exchange them. Those of a slab are loaded while the slab before is computed.
+        const int64_t n = min(n0 + row0 + g + 8 * t, N - 1);   // rows past the last are computed with its scales, and not stored
+        const T* scale_row = scales + n * groups;
+        const uint8_t* zero_row = ZEROS ? zeros + n * groups : nullptr;
+        T scale[4 / FLUSH];
+        uint8_t zero[4 / FLUSH];
         int which[4 / FLUSH], in_group[4 / FLUSH];
         auto load_scales = [&]() {
 #pragma unroll
             for (int f = 0; f < 4 / FLUSH; f++) {
                 const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    scale[f][r] = in ? scale_row[r][which[f]] : T(0.0f);
-                    if (ZEROS) zero[f][r] = in ? zero_row[r][which[f]] : 0;
-                }
+                scale[f] = in ? scale_row[which[f]] : T(0.0f);
+                if (ZEROS) zero[f] = in ? zero_row[which[f]] : 0;
                 for (in_group[f] += SLAB_K; in_group[f] >= group; in_group[f] -= group) which[f]++;
             }
         };
@@ -201,34 +198,35 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
         load_scales();
         for (int i = 0; i < count; i++) {
             const int s = i % STAGES;
-            float by[4 / FLUSH][4];
-            Zero<T> z[ZEROS ? 4 / FLUSH : 1][ZEROS ? 4 : 1];
-            if (!ZEROS) z[0][0].set(8);
+            float by[4 / FLUSH];
+            Zero<T> z[ZEROS ? 4 / FLUSH : 1];
+            if (!ZEROS) z[0].set(8);
 #pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    by[f][r] = to_float(scale[f][r]);
-                    if (ZEROS) z[f][r].set(zero[f][r]);
-                }
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                by[f] = to_float(scale[f]);
+                if (ZEROS) z[f].set(zero[f]);
+            }
             load_scales();
             ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const uint32_t w_at = ring + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
-            const uint32_t x_at = ring + s * STAGE_BYTES + W_BYTES + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
+            const uint8_t* w_at = smem + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
+            const uint8_t* x_at = smem + s * STAGE_BYTES + W_BYTES + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
 #pragma unroll
             for (int f = 0; f < 4 / FLUSH; f++) {
                 float acc[2][NT][4] = {};
+                Zero<T> row_z[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) row_z[r] = ZEROS ? z[ZEROS ? f : 0].of_lane((lane & ~3) | r) : z[0];
 #pragma unroll
                 for (int v = 0; v < FLUSH; v++) {
                     const int u = f * FLUSH + v;
                     uint32_t a[4][4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) unpack(load_shared_u32(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), z[ZEROS ? f : 0][ZEROS ? r : 0], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
+                    for (int r = 0; r < 4; r++) unpack(*reinterpret_cast<const uint32_t*>(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), row_z[r], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        const uint4 x = load_shared_v4(x_at + u * TOKENS * X_BOX_K * 2 + nt * 8 * X_BOX_K * 2);   // row 8 nt + g of X, its k 8 t .. 8 t + 7 of the unit
+                        const uint4 x = *reinterpret_cast<const uint4*>(x_at + u * TOKENS * X_BOX_K * 2 + nt * 8 * X_BOX_K * 2);   // row 8 nt + g of X, its k 8 t .. 8 t + 7 of the unit
                         const uint32_t b0 = __byte_perm(x.x, x.z, 0x5410), b1 = __byte_perm(x.x, x.z, 0x7632);
                         const uint32_t b2 = __byte_perm(x.y, x.w, 0x5410), b3 = __byte_perm(x.y, x.w, 0x7632);
 #pragma unroll
@@ -239,51 +237,54 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
                     }
                 }
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int r = 0; r < 4; r++) {
+                    const float b = __shfl_sync(0xffffffffu, by[f], (lane & ~3) | r);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) total[h][nt][j] += by[f][2 * h + (j >> 1)] * acc[h][nt][j];
+                        for (int j = 0; j < 2; j++) total[r >> 1][nt][2 * (r & 1) + j] += b * acc[r >> 1][nt][2 * (r & 1) + j];
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
         }
     }
 
-    // The two halves of a stage and the CTAs of the cluster, added in that order.
-    __syncthreads();   // the ring is done with: its memory takes the partial sums, [half][row of X][row of the weights]
-    float* sums = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
+    // Every row of X has a CTA of the cluster that adds up its sums: both halves of the warps, CTA by CTA, in that order. Each
+    // warp stores its sums where that CTA will read them.
+    __syncwarp();
+    cluster_wait();   // every CTA of the cluster runs, so its shared memory is there
+    const int tokens = min(TOKENS, M - m0), each = (TOKENS + splits - 1) / splits;
+    float* join = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);   // [CTA][half][row of X, of those this CTA adds up][row of the weights]
     if (warp < CONSUMERS) {
-        float* mine = sums + (warp >> 2) * TOKENS * ROWS + (warp & 3) * 32 + (lane >> 2);
+        const uint32_t mine = smem_u32(join + (split * 2 + (warp >> 2)) * each * ROWS + (warp & 3) * 32 + (lane >> 2));
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int e = 0; e < 2; e++) {
+                const int c = 8 * nt + 2 * (lane & 3) + e;
+                if (c >= tokens) continue;
+                const uint32_t to = map_to_cta(mine + c / splits * ROWS * 4, c % splits);
 #pragma unroll
-                for (int j = 0; j < 4; j++) mine[(8 * nt + 2 * (lane & 3) + (j & 1)) * ROWS + 16 * h + 8 * (j >> 1)] = total[h][nt][j];
+                for (int r = 0; r < 4; r++) store_cluster_f32(to + 8 * r * 4, total[r >> 1][nt][2 * (r & 1) + e]);
+            }
     }
+    __syncwarp();
     cluster_sync_all();
-    const int tokens = min(TOKENS, M - m0);
-    for (int i = threadIdx.x; i < ((tokens - split + splits - 1) / splits) * ROWS; i += THREADS) {
+    for (int i = threadIdx.x; i < (tokens - split + splits - 1) / splits * ROWS; i += THREADS) {
         const int row = i % ROWS, c = i / ROWS * splits + split;
         if (n0 + row >= N) continue;
-        const uint32_t at = smem_u32(&sums[c * ROWS + row]);
         float v = 0.0f;
-        for (int q = 0; q < splits; q++) {
-            const uint32_t theirs = map_to_cta(at, q);
-            v += load_cluster_f32(theirs) + load_cluster_f32(theirs + TOKENS * ROWS * 4);
-        }
+        for (int q = 0; q < 2 * splits; q++) v += join[(q * each + i / ROWS) * ROWS + row];
         store_as(C + (m0 + c) * ldc + n0 + row, v);
     }
     if (!ok && status) atomicExch(status, 1);
-    __syncwarp();
-    cluster_sync_all();   // no CTA leaves while another reads its sums
 }
 
 // ---- many rows of X: the weights unpacked into shared memory for tcgen05.mma ----
 //
 // The weights lie along the accumulator's 128 lanes and up to 256 rows of X along its columns (the width of a tile is the
-// host's choice, a multiple of 16). Per slab of 64 k eight warps turn 4 KB of packed weights into the 16 KB swizzled tile that
+// host's choice, a multiple of 16). Teams of four warps turn the 4 KB of packed weights of 64 k into the 16 KB swizzled tile that
 // the MMA reads, (q - z) * s rounded to X's type: unlike the kernel above, which scales sums, this one scales the operand,
 // because a group's sum would have to leave tensor memory for every group. That is one rounding of half a step a weight, of
 // random sign, beside the one of C: the error of C grows by the root of two.
@@ -291,7 +292,8 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 // cluster shares a tile's K, as above, where there are fewer.
 namespace tall {
 constexpr int TILE_K = 64, W_TILE = ROWS * TILE_K * 2, RAW_BYTES = W_BYTES, MAX_STAGES = 6, MAX_RAW = 4;
-constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, UNPACKERS = 8, FIRST_UNPACKER = 3 + 1, EPILOGUE = 4, FIRST_EPILOGUE = FIRST_UNPACKER + UNPACKERS;
+constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, TEAMS = SLAB_K / TILE_K, TEAM = 4, FIRST_UNPACKER = 4, EPILOGUE = 4;
+constexpr int FIRST_EPILOGUE = FIRST_UNPACKER + TEAMS * TEAM;
 constexpr int TALL_THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE), SMEM_MOST = 231936;
 constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 256;
 
@@ -326,6 +328,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t gave_up;
     const uint32_t raw = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = raw + p.raws * RAW_BYTES;
+    uint8_t* smem = smem_raw + (raw - smem_u32(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
     const int my_tile = blockIdx.x / splits, step = gridDim.x / splits;
@@ -336,12 +339,12 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int s = 0; s < p.stages; s++) {
-            mbar_init(smem_u32(&full_bar[s]), 1 + UNPACKERS);   // the rows of X, and each unpacking warp
+            mbar_init(smem_u32(&full_bar[s]), 1 + TEAM);   // the rows of X, and each warp of the team that unpacks it
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int s = 0; s < p.raws; s++) {
             mbar_init(smem_u32(&raw_full[s]), 1);
-            mbar_init(smem_u32(&raw_empty[s]), UNPACKERS);
+            mbar_init(smem_u32(&raw_empty[s]), TEAMS * TEAM);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(smem_u32(&tfull_bar[b]), 1);
@@ -428,54 +431,74 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             }
         }
     } else if (warp >= FIRST_UNPACKER && warp < FIRST_EPILOGUE) {
-        // This thread: row `row` of the tile, half a slab's k (32 of 64): one 16-byte piece in, four out.
-        const int uw = warp - FIRST_UNPACKER, row = (uw & 3) * 32 + lane, half = uw >> 2, groups = (p.K - 1) / p.group + 1;
+        // Four teams of four warps take the four tiles of a slab of packed weights, so that each has four tiles' time for
+        // the way from its barrier to the MMA's. This thread: row `row`, two 16-byte pieces in, eight out.
+        const int team = (warp - FIRST_UNPACKER) / TEAM, row = (warp & 3) * 32 + lane, groups = (p.K - 1) / p.group + 1;
         const uint32_t row_at = row * 128, turn = row & 7;
-        int s = 0, rs = 0;
-        uint32_t ph = 0, rph = 0;
+        const int groups_a_slab = SLAB_K / p.group, left_a_slab = SLAB_K % p.group;
+        int rs = 0, at = 0;   // `at`: the ring's place of this tile's first 64 k
+        uint32_t rph = 0, ph = 0;
+        const auto forward = [&](int& place, uint32_t& parity, int by) {
+            for (place += by; place >= p.stages; place -= p.stages) parity ^= 1;
+        };
         for (int t = my_tile; t < p.tiles && ok; t += step) {
-            const int n = t % p.tiles_n * ROWS + row;
-            const T* scale_row = scales + (int64_t)(n < p.N ? n : 0) * groups;
-            const uint8_t* zero_row = ZEROS ? zeros + (int64_t)(n < p.N ? n : 0) * groups : nullptr;
-            const int k0 = first * SLAB_K + half * UNIT_K;
-            int which = k0 / p.group, in_group = k0 % p.group;
-            T scale = which < groups ? scale_row[which] : T(0.0f);   // past the end of K: X is zero there, and so is the scale
-            int zero = ZEROS && which < groups ? zero_row[which] : 8;
-            for (int i = 0; i < count; i++) {
-                uint32_t s2;
-                {
-                    const T both[2] = {scale, scale};
-                    s2 = *reinterpret_cast<const uint32_t*>(both);
+            const int64_t n = min(t % p.tiles_n * ROWS + row, p.N - 1);   // rows past the last are unpacked with its scales, and not stored
+            const T* scale_row = scales + n * groups;
+            const uint8_t* zero_row = ZEROS ? zeros + n * groups : nullptr;
+            int which[2], in_group[2], zero[2], place = at;
+            T scale[2];
+            uint32_t parity = ph;
+            forward(place, parity, team);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = first * SLAB_K + team * TILE_K + h * UNIT_K;
+                which[h] = k / p.group, in_group[h] = k % p.group;
+            }
+            const auto load_scales = [&]() {   // past the end of K: X is zero there, and so is the scale
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    scale[h] = which[h] < groups ? scale_row[which[h]] : T(0.0f);
+                    zero[h] = ZEROS && which[h] < groups ? zero_row[which[h]] : 8;
+                    which[h] += groups_a_slab, in_group[h] += left_a_slab;
+                    if (in_group[h] >= p.group) in_group[h] -= p.group, which[h]++;
                 }
-                const uint32_t z2 = zero_of(T(0.0f), zero);
-                for (in_group += TILE_K; in_group >= p.group; in_group -= p.group) which++;   // the next slab's scale, while this one waits
-                scale = which < groups ? scale_row[which] : T(0.0f);
-                if (ZEROS) zero = which < groups ? zero_row[which] : 8;
-                if (i % 4 == 0) {
-                    ok &= mbar_wait(smem_u32(&raw_full[rs]), rph, &gave_up);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+            };
+            load_scales();
+            for (int j = 0; j < slabs_here; j++) {
+                uint32_t s2[2], z2[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const T both[2] = {scale[h], scale[h]};
+                    s2[h] = *reinterpret_cast<const uint32_t*>(both);
+                    z2[h] = zero_of(T(0.0f), zero[h]);
                 }
-                const uint4 w = load_shared_v4(raw + rs * RAW_BYTES + row_at + (((2 * (i % 4) + half) ^ turn) << 4));
-                if (i % 4 == 3 || i == count - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&raw_empty[rs]));
-                    if (++rs == p.raws) rs = 0, rph ^= 1;
-                }
-                const uint4 a = unpack_scaled<T>(w.x, z2, s2), b = unpack_scaled<T>(w.y, z2, s2), c = unpack_scaled<T>(w.z, z2, s2), d = unpack_scaled<T>(w.w, z2, s2);
-                ok &= mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
+                load_scales();   // the next slab's, while this one waits
+                ok &= mbar_wait(smem_u32(&raw_full[rs]), rph, &gave_up);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                const uint32_t to = ring + s * stage_bytes + row_at;
-                store_shared_v4(to + (((4 * half + 0) ^ turn) << 4), a);
-                store_shared_v4(to + (((4 * half + 1) ^ turn) << 4), b);
-                store_shared_v4(to + (((4 * half + 2) ^ turn) << 4), c);
-                store_shared_v4(to + (((4 * half + 3) ^ turn) << 4), d);
+                uint4 out[8];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(smem + rs * RAW_BYTES + row_at + (((2 * team + h) ^ turn) << 4));
+                    out[4 * h] = unpack_scaled<T>(w.x, z2[h], s2[h]), out[4 * h + 1] = unpack_scaled<T>(w.y, z2[h], s2[h]);
+                    out[4 * h + 2] = unpack_scaled<T>(w.z, z2[h], s2[h]), out[4 * h + 3] = unpack_scaled<T>(w.w, z2[h], s2[h]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&raw_empty[rs]));
+                if (++rs == p.raws) rs = 0, rph ^= 1;
+                if (4 * j + team >= count) continue;   // this tile lies behind the end of K
+                ok &= mbar_wait(smem_u32(&empty_bar[place]), parity ^ 1, &gave_up);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint8_t* to = smem + p.raws * RAW_BYTES + place * stage_bytes + row_at;
+#pragma unroll
+                for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(to + ((c ^ turn) << 4)) = out[c];
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads what this thread wrote
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&full_bar[s]));
-                if (++s == p.stages) s = 0, ph ^= 1;
+                if (lane == 0) mbar_arrive(smem_u32(&full_bar[place]));
+                forward(place, parity, TEAMS);
             }
+            forward(at, ph, count);
         }
     } else if (warp >= FIRST_EPILOGUE && splits == 1) {
         const int ew = warp & 3;   // this warp may touch lanes 32 ew .. 32 ew + 31
@@ -508,7 +531,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
 
     if (splits > 1) {   // one tile a cluster: the CTAs' sums, added in the order of the CTAs
         __syncthreads();   // the ring is done with: its memory takes the sums
-        float* sums = reinterpret_cast<float*>(smem_raw + (raw - smem_u32(smem_raw)));
+        float* sums = reinterpret_cast<float*>(smem);
         const int n0 = my_tile % p.tiles_n * ROWS, m0 = my_tile / p.tiles_n * p.tile_m, rows = min(p.tile_m, p.M - m0);
         if (warp >= FIRST_EPILOGUE) {
             const int ew = warp & 3;
@@ -560,7 +583,7 @@ int launch(const Args& p) {
     CUtensorMap mw, mx;
     const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
-    if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, X_BOX_K, 8 * NT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, X_BOX_K, p.M < 8 * NT ? p.M : 8 * NT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
     constexpr auto kern = matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
     constexpr int smem = smem_of<NT>();
     if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
@@ -614,8 +637,8 @@ int launch_tall(const Args& p) {
 
 template <class T>
 int launch_type(const Args& p) {
-    if (p.M > 32 && p.N >= ROWS) return p.zeros ? launch_tall<T, true>(p) : launch_tall<T, false>(p);
-    return p.M <= 8 ? launch_flush<T, 1>(p) : p.M <= 16 ? launch_flush<T, 2>(p) : launch_flush<T, 4>(p);
+    if (p.M > 16 && p.N >= ROWS) return p.zeros ? launch_tall<T, true>(p) : launch_tall<T, false>(p);
+    return p.M <= 8 ? launch_flush<T, 1>(p) : launch_flush<T, 2>(p);
 }
 
 }  // namespace

@@ -202,7 +202,7 @@ int basalt_k_matmul_e4m3(const void *A, int64_t lda, const float *a_scales, cons
 /* C[m, n] = sum_k X[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]: X [M x K] and C [M x N] of `type` (F16 or
  * BF16), W the four-bit q, two to a byte along k (k even in the low half), rows ldw bytes apart; scales s [N x
  * ceil(K / group)] of `type` and zeros z [N x ceil(K / group)] (one byte each, 0 .. 128; NULL: 8 everywhere), both
- * without gaps.  group is a multiple of 32.  Any M, N, K >= 1 (M or N 0 does nothing); X, W and ldw must be
+ * without gaps, from a multiple of 4 bytes.  group is a multiple of 32.  Any M, N, K >= 1 (M or N 0 does nothing); X, W and ldw must be
  * multiples of 16 bytes, ldx of 8 elements.  Sums are f32, C is rounded once.  No workspace, no atomics.  `status` as for
  * basalt_k_matmul_f16. */
 int basalt_k_matmul_w4(int type, const void *X, int64_t ldx, const void *W, int64_t ldw, const void *scales,

@@ -98,6 +98,8 @@ def test_matmul_e4m3_refuses(change, message):
     (dict(ldw=16), "row stride"),
     (dict(ldc=7), "row stride"),
     (dict(Cm=Z + 1), "aligned"),
+    (dict(scales=S + 2), "multiple of 4"),
+    (dict(zeros=W + 1), "multiple of 4"),
     (dict(Cm=X), "overlaps"),
     (dict(Cm=Y), "overlaps"),
 ])
