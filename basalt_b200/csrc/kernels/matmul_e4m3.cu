@@ -54,7 +54,7 @@ __host__ __device__ constexpr int smem_of() {
 template <class T, int TN>
 __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
                                                               const float* __restrict__ a_scales, const float* __restrict__ b_scales, T* __restrict__ C,
-                                                              int64_t ldc, int M, int N, int K, int tiles_n, int32_t* status) {
+                                                              int64_t ldc, int M, int N, int K, int shift, int32_t* status) {
     constexpr int STAGES = stages_of<TN>(), A_BYTES = TN * BK, STAGE_BYTES = B_BYTES + A_BYTES;
     constexpr uint32_t TMEM_COLS = TN < 32 ? 32 : TN;
     extern __shared__ uint8_t smem_raw[];
@@ -63,10 +63,8 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     __shared__ volatile uint32_t gave_up;
     const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
-    const int tile = blockIdx.x / splits, n0 = tile % tiles_n * BN, m0 = tile / tiles_n * TN;
-    const int slabs = (K - 1) / BK + 1;
-    const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
+    const int splits = 1 << shift, split = blockIdx.x & (splits - 1), n0 = (blockIdx.x >> shift) * BN, m0 = blockIdx.y * TN;
+    const int slabs = (K - 1) / BK + 1, first = slabs * split >> shift, count = (slabs * (split + 1) >> shift) - first;
 
     if (threadIdx.x == 0) {
         gave_up = 0;
@@ -366,11 +364,10 @@ int launch(const Args& p) {
     if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
     const int tiles_n = (p.N - 1) / BN + 1, slabs = (p.K - 1) / BK + 1;
     const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TN + 1);
-    int splits = 1;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps four slabs
-    while (splits < 8 && tiles * splits * 2 <= 2 * basalt_k::sm_count() && slabs >= splits * 8) splits *= 2;
-    if (tiles * splits > INT32_MAX) return basalt_k::record_msg(1, WHO, "M * N is too large");
-    return basalt_k::launch_clusters(WHO, kern, (unsigned)(tiles * splits), THREADS, smem, splits, p.stream, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K,
-                                     tiles_n, p.status);
+    int shift = 0;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps four slabs
+    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && slabs >= 8 << shift) shift++;
+    const dim3 grid(tiles_n << shift, (p.M - 1) / TN + 1);   // M is at most 256 here
+    return basalt_k::launch_clusters(WHO, kern, grid, THREADS, smem, 1 << shift, p.stream, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, shift, p.status);
 }
 
 template <class T, bool VECTORS>

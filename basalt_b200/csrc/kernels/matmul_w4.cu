@@ -30,22 +30,50 @@ namespace {
 
 using namespace basalt_k::tc;
 
-constexpr int ROWS = 128, SLAB_K = 256, W_BYTES = ROWS * SLAB_K / 2, CONSUMERS = 8, THREADS = 32 * (CONSUMERS + 1);
-constexpr int UNIT_K = 32, X_BOX_K = 32;   // a unit: the 32 k that one 16-byte piece of a weight row holds
-
-template <int NT>
-__host__ __device__ constexpr int x_bytes_of() { return 8 * NT * SLAB_K * 2; }
-template <int NT>
-__host__ __device__ constexpr int stages_of() { return NT == 1 ? 5 : 3; }
-template <int NT>
-__host__ __device__ constexpr int join_bytes_of() { return 2 * 8 * NT * ROWS * 4; }   // the sums of both halves of the warps, for every row of X
-template <int NT>
-__host__ __device__ constexpr int smem_of() { return stages_of<NT>() * (W_BYTES + x_bytes_of<NT>()) + join_bytes_of<NT>() + 1024; }   // at most 113 KB: two CTAs fit an SM
+constexpr int ROWS = 128, UNIT_K = 32;
 
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// The 4-byte word at `offset` of `from` to shared memory, asynchronously; what lies behind `end` is not read, and arrives as zeros.
+__device__ __forceinline__ void copy_word(uint32_t to, const void* from, int64_t offset, int64_t end) {
+    const int bytes = (int)max((int64_t)0, min((int64_t)4, end - offset));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"((const uint8_t*)from + (bytes ? offset : 0)), "r"(bytes) : "memory");
+}
+// Arrives on the barrier when every copy that this thread has begun is done.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory"); }
+
+// A slab's scales and zero points in shared memory: of each of the tile's 128 rows the groups that 256 k touch, at most 8 / FLUSH where
+// FLUSH * 32 k certainly share a group, as the 4-byte words that hold them. (A load by each thread that wants a scale
+// touches 32 rows, so 32 lines of the cache, in an instruction: with those the unpacking of 64 k took 900 clocks, SCALES_HERE with this.)
+template <class T, int FLUSH, bool ZEROS>
+struct SlabScales {
+    static constexpr int GROUPS = 8 / FLUSH, SCALE_WORDS = GROUPS / 2 + 1, ZERO_WORDS = ZEROS ? (GROUPS + 6) / 4 : 0;
+    static constexpr int ZERO_AT = ROWS * SCALE_WORDS * 4, BYTES = (ZERO_AT + ROWS * ZERO_WORDS * 4 + 1023) / 1024 * 1024;
+
+    // One warp's copies for the rows from n0, beginning with group `start`; `at`: where in shared memory.
+    static __device__ __forceinline__ void copy(uint32_t at, const void* scales, const void* zeros, int n0, int N, int groups, int start, int lane) {
+        const int64_t scale_end = (int64_t)N * groups * 2, zero_end = (int64_t)N * groups;
+#pragma unroll
+        for (int r = 0; r < ROWS / 32; r++) {
+            const int row = lane + 32 * r;
+            const int64_t group = (int64_t)min(n0 + row, N - 1) * groups + start;   // rows past the last get its scales
+#pragma unroll
+            for (int w = 0; w < SCALE_WORDS; w++) copy_word(at + (row * SCALE_WORDS + w) * 4, scales, (group * 2 & ~3LL) + 4 * w, scale_end);
+#pragma unroll
+            for (int w = 0; w < ZERO_WORDS; w++) copy_word(at + ZERO_AT + (row * ZERO_WORDS + w) * 4, zeros, (group & ~3LL) + 4 * w, zero_end);
+        }
+    }
+    // The scale and zero point of row `row` and group start + ahead; row_group: N row's first group, modulo 4 at least.
+    static __device__ __forceinline__ uint32_t scale_bits(const uint8_t* at, int row, uint32_t row_group, int start, int ahead) {
+        return reinterpret_cast<const uint16_t*>(at + row * SCALE_WORDS * 4)[((row_group + start) & 1) + ahead];
+    }
+    static __device__ __forceinline__ int zero(const uint8_t* at, int row, uint32_t row_group, int start, int ahead) {
+        return at[ZERO_AT + row * ZERO_WORDS * 4 + ((row_group + start) & 3) + ahead];
+    }
+};
 
 // (a & mask) | magic in one instruction
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t magic) {
@@ -104,6 +132,10 @@ __device__ __forceinline__ void unpack(uint32_t w, const Zero<__nv_bfloat16>& z,
     }
 }
 
+// The power of two whose last bits of mantissa four bits become: 1024 in f16, 128 in bf16.
+template <class T>
+constexpr uint32_t MAGIC = std::is_same_v<T, __half> ? 0x64006400u : 0x43004300u;
+
 template <class T>
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same_v<T, __half>)
@@ -116,137 +148,187 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: tiles of eight rows of X. FLUSH: units (32 k) that certainly share a group, 1, 2 or 4.
-template <class T, int NT, int FLUSH, bool ZEROS>
-__global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                                                               const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C, int64_t ldc,
-                                                               int M, int N, int K, int group, int tiles_n, int32_t* status) {
-    constexpr int STAGES = stages_of<NT>(), TOKENS = 8 * NT, X_BYTES = x_bytes_of<NT>(), STAGE_BYTES = W_BYTES + X_BYTES;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
-    __shared__ volatile uint32_t gave_up;
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* smem = smem_raw + (ring - smem_u32(smem_raw));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
-    const int tile = blockIdx.x / splits, n0 = tile % tiles_n * ROWS, m0 = tile / tiles_n * TOKENS;
-    const int slabs = (K - 1) / SLAB_K + 1;
-    const int first = (int)((int64_t)slabs * split / splits), count = (int)((int64_t)slabs * (split + 1) / splits) - first;
+// ---- few rows of X ----
+//
+// A CTA takes 128 rows of the weights over its share of K, in blocks of 128 k: four groups of 32 rows, the even and the odd blocks by
+// a warp each. A warp loads its weights from global memory straight into the registers it unpacks, 64 bytes of 32 rows a block,
+// and keeps DEEP blocks in flight; nothing but X goes through shared memory, where it lies in the order in which the
+// instructions want it, and no barrier stands in the loop.
+// (Through a ring of bulk loads the same sums took 12.7 us where this takes TIME_HERE, 8192 x 8192 for one row: the barriers and
+// addresses of each slab cost a third of its instructions.)
+namespace few {
+constexpr int BLOCK_K = 128, WARPS = 8, THREADS = 32 * WARPS, X_BYTES = 64 * 1024;
 
-    if (threadIdx.x == 0) {
-        prefetch_map(&map_w);
-        prefetch_map(&map_x);
-        gave_up = 0;
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(smem_u32(&full_bar[s]), 1);
-            mbar_init(smem_u32(&empty_bar[s]), CONSUMERS);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    __syncthreads();
+template <int NT>
+struct Tile {
+    static constexpr int TOKENS = 8 * NT, DEEP = NT == 1 ? 3 : 2, JOIN = 2 * TOKENS * ROWS * 4;
+    static constexpr int ROUND = 2 * DEEP;   // blocks in which both warps have gone once through their registers' DEEP places
+    static constexpr int X_BLOCKS = X_BYTES / (TOKENS * BLOCK_K * 2) / ROUND * ROUND;
+    static constexpr int SMEM = X_BYTES + JOIN;   // at most 96 KB: two CTAs fit an SM
+};
+
+// Where lane t of four finds word j of its weights in a block, in 8-k words: FLUSH words of the four lanes together hold k's that
+// certainly share a group (FLUSH * 32 of them).
+template <int FLUSH>
+__device__ __forceinline__ constexpr int word_of(int t, int j) { return FLUSH == 4 ? 4 * t + j : FLUSH == 2 ? 8 * (j >> 1) + 2 * t + (j & 1) : 4 * j + t; }
+
+template <class T, int FLUSH, bool ZEROS>
+struct Block {
+    uint32_t w[4][4];   // [row g + 8 r][word]
+    T scale[4 / FLUSH];
+    uint8_t zero[4 / FLUSH];
+};
+
+// `valid` bytes of four words; what lies behind is not read.
+__device__ __noinline__ uint32_t partial_word(const uint8_t* p, int valid) {
+    uint32_t v = 0;
+    for (int i = 0; i < valid && i < 4; i++) v |= (uint32_t)p[i] << (8 * i);
+    return v;
+}
+__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+struct Shape {
+    const uint8_t* w;
+    const void *x, *scales;
+    const uint8_t* zeros;
+    void* c;
+    int64_t ldw, ldx, ldc;
+    int M, N, K, group, groups, split_shift;   // a tile's K is shared by 1 << split_shift CTAs
+};
+
+template <class T, int NT, int FLUSH, bool ZEROS>
+__global__ void __launch_bounds__(THREADS, 2) matmul_w4_few(const Shape p) {
+    using S = Tile<NT>;
+    constexpr int TOKENS = S::TOKENS, DEEP = S::DEEP, FLUSHES = 4 / FLUSH;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
+    // (No division of the prologue is done that the host can do: on the way to the first load their latencies add up.)
+    const int shift = p.split_shift, splits = 1 << shift, split = blockIdx.x & (splits - 1), groups = p.groups, row_bytes = (p.K + 1) / 2;
+    const int n0 = (blockIdx.x >> shift) * ROWS, m0 = blockIdx.y * TOKENS, tokens = min(TOKENS, p.M - m0);
+    const int blocks = (p.K - 1) / BLOCK_K + 1, first = blocks * split >> shift, last = blocks * (split + 1) >> shift;
     cluster_arrive();
     wait_for_predecessor();
-    if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
-    bool ok = true;
-    float total[2][NT][4] = {};
 
-    if (warp == CONSUMERS) {
-        if (lane == 0) {
-            for (int i = 0; i < count; i++) {
-                const int s = i % STAGES;
-                ok &= mbar_wait(smem_u32(&empty_bar[s]), ((i / STAGES) & 1) ^ 1, &gave_up);
-                if (!ok) break;
-                const uint32_t fb = smem_u32(&full_bar[s]), w_dst = ring + s * STAGE_BYTES, x_dst = w_dst + W_BYTES;
-                const int k = (first + i) * SLAB_K;
-                mbar_expect_tx(fb, W_BYTES + min(M, TOKENS) * SLAB_K * 2);
-                tma_load_2d(w_dst, &map_w, fb, k / 2, n0);
+    const uint8_t* w_row[4];   // this lane's part of rows g, g + 8, g + 16 and g + 24; rows past the last are computed with its weights, and not stored
 #pragma unroll
-                for (int b = 0; b < SLAB_K / X_BOX_K; b++) tma_load_2d(x_dst + b * TOKENS * X_BOX_K * 2, &map_x, fb, k + b * X_BOX_K, m0);
+    for (int r = 0; r < 4; r++) w_row[r] = p.w + (int64_t)min(n0 + row0 + g + 8 * r, p.N - 1) * p.ldw + 4 * word_of<FLUSH>(t, 0);
+    // Of those four rows, which four lanes share, lane t loads the scales of row g + 8 t, and the lanes exchange them.
+    const int64_t my_row = (int64_t)min(n0 + row0 + g + 8 * t, p.N - 1) * groups;
+    const T* scale_row = (const T*)p.scales + my_row;
+    const uint8_t* zero_row = ZEROS ? p.zeros + my_row : nullptr;
+    int which[FLUSHES], in_group[FLUSHES];   // the groups of the next block to load, and where in them its parts begin
+    which[0] = (unsigned)((first + half) * BLOCK_K) / (unsigned)p.group, in_group[0] = (first + half) * BLOCK_K - which[0] * p.group;
+#pragma unroll
+    for (int f = 1; f < FLUSHES; f++) {
+        which[f] = which[f - 1], in_group[f] = in_group[f - 1] + FLUSH * UNIT_K;
+        if (in_group[f] >= p.group) in_group[f] -= p.group, which[f]++;
+    }
+    const auto load = [&](Block<T, FLUSH, ZEROS>& b, int block) {
+        if (block >= last) return;
+        const int at = block * (BLOCK_K / 2);
+        if (at + BLOCK_K / 2 <= row_bytes) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint8_t* q = w_row[r] + at;
+                if constexpr (FLUSH == 4) {
+                    const uint4 v = load_stream(q);
+                    b.w[r][0] = v.x, b.w[r][1] = v.y, b.w[r][2] = v.z, b.w[r][3] = v.w;
+                } else if constexpr (FLUSH == 2) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(q)), u = __ldg(reinterpret_cast<const uint2*>(q + 32));
+                    b.w[r][0] = v.x, b.w[r][1] = v.y, b.w[r][2] = u.x, b.w[r][3] = u.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) b.w[r][j] = __ldg(reinterpret_cast<const uint32_t*>(q + 16 * j));
+                }
             }
-            if (!ok) {   // let the copies already issued land before the CTA can exit
-                const uint64_t t0 = global_ns();
-                while (global_ns() - t0 < 2000000ull) {}
-            }
+        } else {   // the block in which the rows end
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int ahead = 4 * (word_of<FLUSH>(t, j) - word_of<FLUSH>(t, 0));
+                    b.w[r][j] = partial_word(w_row[r] + at + ahead, row_bytes - at - 4 * word_of<FLUSH>(t, j));
+                }
         }
-        __syncwarp();
-    } else {
-        const int half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
-        const int groups = (K - 1) / group + 1;
-        // Of the four weight rows g, g + 8, g + 16 and g + 24 that four lanes share, lane t loads the scales of row g + 8 t and the
-        // lanes exchange them. Those of a slab are loaded while the slab before is computed.
-        const int64_t n = min(n0 + row0 + g + 8 * t, N - 1);   // rows past the last are computed with its scales, and not stored
-        const T* scale_row = scales + n * groups;
-        const uint8_t* zero_row = ZEROS ? zeros + n * groups : nullptr;
-        T scale[4 / FLUSH];
-        uint8_t zero[4 / FLUSH];
-        int which[4 / FLUSH], in_group[4 / FLUSH];
-        auto load_scales = [&]() {
 #pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++) {
-                const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
-                scale[f] = in ? scale_row[which[f]] : T(0.0f);
-                if (ZEROS) zero[f] = in ? zero_row[which[f]] : 0;
-                for (in_group[f] += SLAB_K; in_group[f] >= group; in_group[f] -= group) which[f]++;
-            }
-        };
-#pragma unroll
-        for (int f = 0; f < 4 / FLUSH; f++) {
-            const int k = first * SLAB_K + half * 128 + f * FLUSH * UNIT_K;
-            which[f] = k / group, in_group[f] = k % group;
+        for (int f = 0; f < FLUSHES; f++) {
+            const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
+            b.scale[f] = in ? scale_row[which[f]] : T(0.0f);
+            if (ZEROS) b.zero[f] = in ? zero_row[which[f]] : 0;
+            for (in_group[f] += 2 * BLOCK_K; in_group[f] >= p.group; in_group[f] -= p.group) which[f]++;
         }
-        load_scales();
-        for (int i = 0; i < count; i++) {
-            const int s = i % STAGES;
-            float by[4 / FLUSH];
-            Zero<T> z[ZEROS ? 4 / FLUSH : 1];
-            if (!ZEROS) z[0].set(8);
+    };
+
+    float total[2][NT][4] = {};
+    const auto compute = [&](const Block<T, FLUSH, ZEROS>& b, int block_here) {
+        const uint8_t* x_at = smem + block_here * (4 * TOKENS * 64) + lane * 16;
 #pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++) {
-                by[f] = to_float(scale[f]);
-                if (ZEROS) z[f].set(zero[f]);
-            }
-            load_scales();
-            ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const uint8_t* w_at = smem + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
-            const uint8_t* x_at = smem + s * STAGE_BYTES + W_BYTES + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
+        for (int f = 0; f < FLUSHES; f++) {
+            Zero<T> z, row_z[4];
+            z.set(ZEROS ? b.zero[f] : 8);
 #pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++) {
-                float acc[2][NT][4] = {};
-                Zero<T> row_z[4];
+            for (int r = 0; r < 4; r++) row_z[r] = ZEROS ? z.of_lane((lane & ~3) | r) : z;
+            float acc[2][NT][4] = {};
 #pragma unroll
-                for (int r = 0; r < 4; r++) row_z[r] = ZEROS ? z[ZEROS ? f : 0].of_lane((lane & ~3) | r) : z[0];
+            for (int v = 0; v < FLUSH; v++) {
+                const int j = f * FLUSH + v;
+                uint32_t a[4][4];
 #pragma unroll
-                for (int v = 0; v < FLUSH; v++) {
-                    const int u = f * FLUSH + v;
-                    uint32_t a[4][4];
+                for (int r = 0; r < 4; r++) unpack(b.w[r][j], row_z[r], a[r]);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) unpack(*reinterpret_cast<const uint32_t*>(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), row_z[r], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(x_at + (j * TOKENS + 8 * nt) * 64);   // row 8 nt + g of X, the k's of word j of lane t
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(x_at + u * TOKENS * X_BOX_K * 2 + nt * 8 * X_BOX_K * 2);   // row 8 nt + g of X, its k 8 t .. 8 t + 7 of the unit
-                        const uint32_t b0 = __byte_perm(x.x, x.z, 0x5410), b1 = __byte_perm(x.x, x.z, 0x7632);
-                        const uint32_t b2 = __byte_perm(x.y, x.w, 0x5410), b3 = __byte_perm(x.y, x.w, 0x7632);
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            mma_16816<T>(acc[h][nt], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], b0, b1);
-                            mma_16816<T>(acc[h][nt], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], b2, b3);
-                        }
+                    for (int h = 0; h < 2; h++) {
+                        mma_16816<T>(acc[h][nt], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
+                        mma_16816<T>(acc[h][nt], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x.z, x.w);
                     }
                 }
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float b = __shfl_sync(0xffffffffu, by[f], (lane & ~3) | r);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int j = 0; j < 2; j++) total[r >> 1][nt][2 * (r & 1) + j] += b * acc[r >> 1][nt][2 * (r & 1) + j];
-                }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
+            const float my_scale = to_float(b.scale[f]);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float row_scale = __shfl_sync(0xffffffffu, my_scale, (lane & ~3) | r);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) total[r >> 1][nt][2 * (r & 1) + j] += row_scale * acc[r >> 1][nt][2 * (r & 1) + j];
+            }
+        }
+    };
+
+    Block<T, FLUSH, ZEROS> b[DEEP];
+#pragma unroll
+    for (int d = 0; d < DEEP; d++) load(b[d], first + half + 2 * d);
+    for (int from = first; from < last; from += S::X_BLOCKS) {   // as many blocks of X as shared memory takes
+        const int to = min(from + S::X_BLOCKS, last), pieces = (to - from) * (BLOCK_K / 8);
+        if (from != first) __syncthreads();   // the blocks before have been computed
+        for (int m = 0; m < tokens; m++)
+        for (int q = threadIdx.x; q < pieces; q += THREADS) {   // eight k of a row of X each, in the order of the pairs that unpack() makes
+            const int word = q % 16, k = from * BLOCK_K + q * 8;
+            const T* x = (const T*)p.x + (m0 + m) * p.ldx + k;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (k + 8 <= p.K) v = __ldg(reinterpret_cast<const uint4*>(x));
+            else if (k < p.K) {
+                uint32_t e[4] = {0, 0, 0, 0};
+                for (int c = 0; c < p.K - k; c++) e[c / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[c] << (16 * (c % 2));
+                v = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+            const int wt = FLUSH == 4 ? word >> 2 : FLUSH == 2 ? (word & 7) >> 1 : word & 3, wj = FLUSH == 4 ? word & 3 : FLUSH == 2 ? (word >> 3) * 2 + (word & 1) : word >> 2;
+            *reinterpret_cast<uint4*>(smem + (((q / 16) * 4 + wj) * TOKENS + m) * 64 + wt * 16) =
+                make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        }
+        __syncthreads();
+        for (int block = from + half; block < to; block += 2 * DEEP) {
+#pragma unroll
+            for (int d = 0; d < DEEP; d++) {
+                if (block + 2 * d < to) compute(b[d], block + 2 * d - from);
+                if (block + 2 * d < to) load(b[d], block + 2 * (d + DEEP));
+            }
         }
     }
 
@@ -254,32 +336,30 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     // warp stores its sums where that CTA will read them.
     __syncwarp();
     cluster_wait();   // every CTA of the cluster runs, so its shared memory is there
-    const int tokens = min(TOKENS, M - m0), each = (TOKENS + splits - 1) / splits;
-    float* join = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);   // [CTA][half][row of X, of those this CTA adds up][row of the weights]
-    if (warp < CONSUMERS) {
-        const uint32_t mine = smem_u32(join + (split * 2 + (warp >> 2)) * each * ROWS + (warp & 3) * 32 + (lane >> 2));
+    const int each = TOKENS >> shift;
+    float* join = reinterpret_cast<float*>(smem + X_BYTES);   // [CTA][half][row of X, of those this CTA adds up][row of the weights]
+    const uint32_t mine = smem_u32(join + (split * 2 + half) * each * ROWS + row0 + g);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int c = 8 * nt + 2 * (lane & 3) + e;
-                if (c >= tokens) continue;
-                const uint32_t to = map_to_cta(mine + c / splits * ROWS * 4, c % splits);
+        for (int e = 0; e < 2; e++) {
+            const int c = 8 * nt + 2 * t + e;
+            if (c >= tokens) continue;
+            const uint32_t to = map_to_cta(mine + (c >> shift) * ROWS * 4, c & (splits - 1));
 #pragma unroll
-                for (int r = 0; r < 4; r++) store_cluster_f32(to + 8 * r * 4, total[r >> 1][nt][2 * (r & 1) + e]);
-            }
-    }
+            for (int r = 0; r < 4; r++) store_cluster_f32(to + 8 * r * 4, total[r >> 1][nt][2 * (r & 1) + e]);
+        }
     __syncwarp();
     cluster_sync_all();
-    for (int i = threadIdx.x; i < (tokens - split + splits - 1) / splits * ROWS; i += THREADS) {
-        const int row = i % ROWS, c = i / ROWS * splits + split;
-        if (n0 + row >= N) continue;
+    for (int i = threadIdx.x; i < ((tokens - split + splits - 1) >> shift) * ROWS; i += THREADS) {
+        const int row = i % ROWS, c = (i / ROWS << shift) + split;
+        if (n0 + row >= p.N) continue;
         float v = 0.0f;
         for (int q = 0; q < 2 * splits; q++) v += join[(q * each + i / ROWS) * ROWS + row];
-        store_as(C + (m0 + c) * ldc + n0 + row, v);
+        store_as((T*)p.c + (m0 + c) * p.ldc + n0 + row, v);
     }
-    if (!ok && status) atomicExch(status, 1);
 }
+}  // namespace few
 
 // ---- many rows of X: the weights unpacked into shared memory for tcgen05.mma ----
 //
@@ -291,38 +371,35 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 // Persistent where there are more tiles than SMs (two accumulators: a tile's stores hide behind the next one's products); a
 // cluster shares a tile's K, as above, where there are fewer.
 namespace tall {
-constexpr int TILE_K = 64, W_TILE = ROWS * TILE_K * 2, RAW_BYTES = W_BYTES, MAX_STAGES = 6, MAX_RAW = 4;
+constexpr int SLAB_K = 256, TILE_K = 64, PACKED_BYTES = ROWS * SLAB_K / 2, MAX_STAGES = 8, MAX_RAW = 4, MAX_M = 256;
 constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, TEAMS = SLAB_K / TILE_K, TEAM = 4, FIRST_UNPACKER = 4, EPILOGUE = 4;
 constexpr int FIRST_EPILOGUE = FIRST_UNPACKER + TEAMS * TEAM;
 constexpr int TALL_THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE), SMEM_MOST = 231936;
-constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 256;
+// Tensor memory: 256 columns of accumulators (two of up to 128, or one), and 32 columns a stage for 64 k of unpacked weights.
+constexpr uint32_t TMEM_COLS = 512, WEIGHTS_AT = 256, WEIGHT_COLS = TILE_K / 2;
 
 // Eight packed weights of one group -> (q - z) * s in the order of k, two to a register.
 template <class T>
-__device__ __forceinline__ uint4 unpack_scaled(uint32_t w, uint32_t zero, uint32_t scale) {
-    constexpr uint32_t MAGIC = std::is_same_v<T, __half> ? 0x64006400u : 0x43004300u;
+__device__ __forceinline__ void unpack_scaled(uint32_t w, uint32_t zero, uint32_t scale, uint32_t* p) {
     using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
     const uint32_t up = w >> 4;
-    uint32_t p[4];
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-        const uint32_t v = and_or(__byte_perm(w, up, b | (4 + b) << 8), 0x000F000Fu, MAGIC);
+        const uint32_t v = and_or(__byte_perm(w, up, b | (4 + b) << 8), 0x000F000Fu, MAGIC<T>);
         const T2 a = __hmul2(__hsub2(*reinterpret_cast<const T2*>(&v), *reinterpret_cast<const T2*>(&zero)), *reinterpret_cast<const T2*>(&scale));
         p[b] = *reinterpret_cast<const uint32_t*>(&a);
     }
-    return make_uint4(p[0], p[1], p[2], p[3]);
 }
-__device__ __forceinline__ uint32_t zero_of(__half, int z) { return 0x00010001u * __half_as_ushort(__int2half_rn(1024 + z)); }
-__device__ __forceinline__ uint32_t zero_of(__nv_bfloat16, int z) { return 0x00010001u * __bfloat16_as_ushort(__int2bfloat16_rn(128 + z)); }
-
 struct Shape {
-    int M, N, K, group, tile_m, tiles_n, tiles, stages, raws;
+    int M, N, K, group, tile_m, tiles_n, tiles, stages, raws, groups, split_shift;
 };
 
-template <class T, bool ZEROS>
+template <class T, int FLUSH, bool ZEROS>
 __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                   const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C,
                                                                   int64_t ldc, const Shape p, int32_t* status) {
+    using Scales = SlabScales<T, FLUSH, ZEROS>;
+    constexpr int RAW_BYTES = PACKED_BYTES + Scales::BYTES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], raw_full[MAX_RAW], raw_empty[MAX_RAW], tfull_bar[2], tempty_bar[2];
     __shared__ uint32_t tmem_slot;
@@ -330,11 +407,12 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     const uint32_t raw = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = raw + p.raws * RAW_BYTES;
     uint8_t* smem = smem_raw + (raw - smem_u32(smem_raw));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = (int)cluster_ctarank(), splits = (int)cluster_nctarank();
-    const int my_tile = blockIdx.x / splits, step = gridDim.x / splits;
-    const int slabs = (p.K - 1) / SLAB_K + 1, first = (int)((int64_t)slabs * split / splits), slabs_here = (int)((int64_t)slabs * (split + 1) / splits) - first;
+    const int shift = p.split_shift, splits = 1 << shift, split = blockIdx.x & (splits - 1);
+    const int my_tile = blockIdx.x >> shift, step = gridDim.x >> shift;
+    const int slabs = (p.K - 1) / SLAB_K + 1, first = slabs * split >> shift, slabs_here = (slabs * (split + 1) >> shift) - first;
     const int count = min(slabs_here * (SLAB_K / TILE_K), (p.K - 1) / TILE_K + 1 - first * (SLAB_K / TILE_K));   // tiles of 64 k
-    const int x_bytes = p.tile_m * TILE_K * 2, stage_bytes = W_TILE + x_bytes;
+    const int first_group = (unsigned)(first * SLAB_K) / (unsigned)p.group;
+    const int stage_bytes = p.tile_m * TILE_K * 2, accs = p.tile_m <= 128 ? 2 : 1;   // with one accumulator, its drain is not hidden
 
     if (threadIdx.x == 0) {
         gave_up = 0;
@@ -343,7 +421,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int s = 0; s < p.raws; s++) {
-            mbar_init(smem_u32(&raw_full[s]), 1);
+            mbar_init(smem_u32(&raw_full[s]), 1 + 32);   // the bulk load, and each lane's copies of scales
             mbar_init(smem_u32(&raw_empty[s]), TEAMS * TEAM);
         }
         for (int b = 0; b < 2; b++) {
@@ -372,11 +450,11 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             for (int t = my_tile; t < p.tiles && ok; t += step) {
                 const int m0 = t / p.tiles_n * p.tile_m;
                 for (int i = 0; i < count; i++) {
-                    ok &= mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
+                    ok &= mbar_wait<LONG_WAIT>(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
                     if (!ok) break;
                     const uint32_t fb = smem_u32(&full_bar[s]);
-                    mbar_expect_tx(fb, x_bytes);
-                    tma_load_2d(ring + s * stage_bytes + W_TILE, &map_x, fb, first * SLAB_K + i * TILE_K, m0);
+                    mbar_expect_tx(fb, stage_bytes);
+                    tma_load_2d(ring + s * stage_bytes, &map_x, fb, first * SLAB_K + i * TILE_K, m0);
                     if (++s == p.stages) s = 0, ph ^= 1;
                 }
             }
@@ -386,102 +464,107 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             }
         }
     } else if (warp == WARP_RAW) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            for (int t = my_tile; t < p.tiles && ok; t += step) {
-                const int n0 = t % p.tiles_n * ROWS;
-                for (int i = 0; i < slabs_here; i++) {
-                    ok &= mbar_wait(smem_u32(&raw_empty[s]), ph ^ 1, &gave_up);
-                    if (!ok) break;
-                    const uint32_t fb = smem_u32(&raw_full[s]);
-                    mbar_expect_tx(fb, RAW_BYTES);
-                    tma_load_2d(raw + s * RAW_BYTES, &map_w, fb, (first + i) * SLAB_K / 2, n0);
-                    if (++s == p.raws) s = 0, ph ^= 1;
+        int s = 0;
+        uint32_t ph = 0;
+        for (int t = my_tile; t < p.tiles && ok; t += step) {
+            const int n0 = t % p.tiles_n * ROWS;
+            int start = first_group, in_group = first * SLAB_K - start * p.group;
+            for (int i = 0; i < slabs_here; i++) {
+                ok &= mbar_wait<LONG_WAIT>(smem_u32(&raw_empty[s]), ph ^ 1, &gave_up);
+                if (!ok) break;
+                const uint32_t fb = smem_u32(&raw_full[s]), at = raw + s * RAW_BYTES;
+                if (lane == 0) {
+                    mbar_expect_tx(fb, PACKED_BYTES);
+                    tma_load_2d(at, &map_w, fb, (first + i) * SLAB_K / 2, n0);
                 }
-            }
-            if (!ok) {
-                const uint64_t t0 = global_ns();
-                while (global_ns() - t0 < 2000000ull) {}
+                Scales::copy(at + PACKED_BYTES, scales, zeros, n0, p.N, p.groups, start, lane);
+                copies_arrive(fb);
+                for (in_group += SLAB_K; in_group >= p.group; in_group -= p.group) start++;
+                if (++s == p.raws) s = 0, ph ^= 1;
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok) {
+            const uint64_t t0 = global_ns();
+            while (global_ns() - t0 < 2000000ull) {}
+        }
     } else if (warp == WARP_MMA) {
-        if (lane == 0) {
-            const uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
-            const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.tile_m >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-            int s = 0;
-            uint32_t ph = 0, local = 0;
-            for (int t = my_tile; t < p.tiles && ok; t += step, local++) {
-                const uint32_t buf = local & 1, use = local >> 1;
-                ok &= mbar_wait(smem_u32(&tempty_bar[buf]), (use & 1) ^ 1, &gave_up);
+        // The warp stays together (see umma_f16_tmem): it shares its scheduler with warps that unpack, and every instruction waits its turn.
+        const uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
+        const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.tile_m >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+        const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
+        const uint64_t x0 = smem_desc(ring, 16, 1024), x_step = stage_bytes >> 4;
+        uint32_t s = 0, ph = 0, buf = 0, use = 0;
+        for (int t = my_tile; t < p.tiles && ok; t += step) {
+            ok &= mbar_wait(smem_u32(&tempty_bar[buf]), (use & 1) ^ 1, &gave_up);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t acc = tmem_base + buf * 128;
+            for (int i = 0; i < count; i++) {
+                ok &= mbar_wait(full0 + 8 * s, ph, &gave_up);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int i = 0; i < count; i++) {
-                    ok &= mbar_wait(smem_u32(&full_bar[s]), ph, &gave_up);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t w_src = ring + s * stage_bytes;
-                    const uint64_t dw = smem_desc(w_src, 16, 1024), dx = smem_desc(w_src + W_TILE, 16, 1024);
+                const uint32_t w = tmem_base + WEIGHTS_AT + s * WEIGHT_COLS;
+                const uint64_t x = x0 + s * x_step;
+                umma_f16_tmem(acc, w, x, idesc, i != 0);
 #pragma unroll
-                    for (int k = 0; k < TILE_K / 16; k++) umma_f16(tmem_base + buf * ACC_COLS, dw + (uint64_t)(2 * k), dx + (uint64_t)(2 * k), idesc, (i | k) != 0);
-                    umma_commit(smem_u32(&empty_bar[s]));
-                    if (++s == p.stages) s = 0, ph ^= 1;
-                }
-                umma_commit(smem_u32(&tfull_bar[buf]));
+                for (int k = 1; k < TILE_K / 16; k++) umma_f16_tmem(acc, w + 8 * k, x + (uint64_t)(2 * k), idesc, 1);
+                umma_commit_elected(empty0 + 8 * s);
+                if (++s == (uint32_t)p.stages) s = 0, ph ^= 1;
             }
+            umma_commit_elected(smem_u32(&tfull_bar[buf]));
+            if (++buf == (uint32_t)accs) buf = 0, use++;
         }
     } else if (warp >= FIRST_UNPACKER && warp < FIRST_EPILOGUE) {
         // Four teams of four warps take the four tiles of a slab of packed weights, so that each has four tiles' time for
-        // the way from its barrier to the MMA's. This thread: row `row`, two 16-byte pieces in, eight out.
-        const int team = (warp - FIRST_UNPACKER) / TEAM, row = (warp & 3) * 32 + lane, groups = (p.K - 1) / p.group + 1;
+        // the way from its barrier to the MMA's. This thread: row `row`, two 16-byte pieces in, its lane's 32 columns out.
+        const int team = (warp - FIRST_UNPACKER) / TEAM, row = (warp & 3) * 32 + lane, groups = p.groups;
         const uint32_t row_at = row * 128, turn = row & 7;
-        const int groups_a_slab = SLAB_K / p.group, left_a_slab = SLAB_K % p.group;
-        int rs = 0, at = 0;   // `at`: the ring's place of this tile's first 64 k
+        constexpr int PARTS = FLUSH == 1 ? 2 : 1;   // groups that 64 k may touch
+        const bool whole = p.group <= SLAB_K && SLAB_K % p.group == 0;
+        const int whole_shift = p.group == 32 ? 0 : p.group == 64 ? 1 : p.group == 128 ? 2 : 3;
+        int steady[PARTS];   // groups from the slab's first to this thread's, where all slabs begin with a group
+#pragma unroll
+        for (int h = 0; h < PARTS; h++) steady[h] = (team * 2 + h) >> whole_shift;
+        int rs = 0, at = 0;                         // `at`: the ring's place of this tile's first 64 k
         uint32_t rph = 0, ph = 0;
         const auto forward = [&](int& place, uint32_t& parity, int by) {
             for (place += by; place >= p.stages; place -= p.stages) parity ^= 1;
         };
         for (int t = my_tile; t < p.tiles && ok; t += step) {
-            const int64_t n = min(t % p.tiles_n * ROWS + row, p.N - 1);   // rows past the last are unpacked with its scales, and not stored
-            const T* scale_row = scales + n * groups;
-            const uint8_t* zero_row = ZEROS ? zeros + n * groups : nullptr;
-            int which[2], in_group[2], zero[2], place = at;
-            T scale[2];
+            const uint32_t row_group = (uint32_t)min(t % p.tiles_n * ROWS + row, p.N - 1) * (uint32_t)groups;
+            int place = at, start = first_group, in_start = first * SLAB_K - start * p.group;
             uint32_t parity = ph;
             forward(place, parity, team);
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int k = first * SLAB_K + team * TILE_K + h * UNIT_K;
-                which[h] = k / p.group, in_group[h] = k % p.group;
-            }
-            const auto load_scales = [&]() {   // past the end of K: X is zero there, and so is the scale
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    scale[h] = which[h] < groups ? scale_row[which[h]] : T(0.0f);
-                    zero[h] = ZEROS && which[h] < groups ? zero_row[which[h]] : 8;
-                    which[h] += groups_a_slab, in_group[h] += left_a_slab;
-                    if (in_group[h] >= p.group) in_group[h] -= p.group, which[h]++;
-                }
-            };
-            load_scales();
             for (int j = 0; j < slabs_here; j++) {
-                uint32_t s2[2], z2[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const T both[2] = {scale[h], scale[h]};
-                    s2[h] = *reinterpret_cast<const uint32_t*>(both);
-                    z2[h] = zero_of(T(0.0f), zero[h]);
-                }
-                load_scales();   // the next slab's, while this one waits
                 ok &= mbar_wait(smem_u32(&raw_full[rs]), rph, &gave_up);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint4 out[8];
+                const uint8_t* stage = smem + rs * RAW_BYTES;
+                uint32_t s2[2], z2[2];
+#pragma unroll
+                for (int h = 0; h < PARTS; h++) {
+                    int ahead = steady[h];
+                    if (!whole) {   // groups that do not divide a slab
+                        ahead = 0;
+                        for (int k = in_start + team * TILE_K + h * UNIT_K; k >= p.group; k -= p.group) ahead++;
+                    }
+                    const bool in = start + ahead < groups;   // past the end of K: X is zero there, and so is the scale
+                    const uint32_t scale = Scales::scale_bits(stage + PACKED_BYTES, row, row_group, start, ahead);
+                    s2[h] = in ? scale * 0x10001u : 0u;
+                    z2[h] = MAGIC<T> + 0x10001u * (ZEROS && in ? Scales::zero(stage + PACKED_BYTES, row, row_group, start, ahead) : 8);
+                }
+                if (PARTS == 1) s2[1] = s2[0], z2[1] = z2[0];
+                if (whole) start += SLAB_K / 32 >> whole_shift;
+                else for (in_start += SLAB_K; in_start >= p.group; in_start -= p.group) start++;
+                uint32_t out[32];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(smem + rs * RAW_BYTES + row_at + (((2 * team + h) ^ turn) << 4));
-                    out[4 * h] = unpack_scaled<T>(w.x, z2[h], s2[h]), out[4 * h + 1] = unpack_scaled<T>(w.y, z2[h], s2[h]);
-                    out[4 * h + 2] = unpack_scaled<T>(w.z, z2[h], s2[h]), out[4 * h + 3] = unpack_scaled<T>(w.w, z2[h], s2[h]);
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + row_at + (((2 * team + h) ^ turn) << 4));
+                    unpack_scaled<T>(w.x, z2[h], s2[h], out + 16 * h), unpack_scaled<T>(w.y, z2[h], s2[h], out + 16 * h + 4);
+                    unpack_scaled<T>(w.z, z2[h], s2[h], out + 16 * h + 8), unpack_scaled<T>(w.w, z2[h], s2[h], out + 16 * h + 12);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&raw_empty[rs]));
@@ -490,10 +573,9 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                 ok &= mbar_wait(smem_u32(&empty_bar[place]), parity ^ 1, &gave_up);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint8_t* to = smem + p.raws * RAW_BYTES + place * stage_bytes + row_at;
-#pragma unroll
-                for (int c = 0; c < 8; c++) *reinterpret_cast<uint4*>(to + ((c ^ turn) << 4)) = out[c];
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the MMA reads what this thread wrote
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tmem_store_32(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + WEIGHTS_AT + place * WEIGHT_COLS, out);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&full_bar[place]));
                 forward(place, parity, TEAMS);
@@ -502,15 +584,14 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
         }
     } else if (warp >= FIRST_EPILOGUE && splits == 1) {
         const int ew = warp & 3;   // this warp may touch lanes 32 ew .. 32 ew + 31
-        uint32_t local = 0;
-        for (int t = my_tile; t < p.tiles && ok; t += step, local++) {
-            const uint32_t buf = local & 1, use = local >> 1;
+        uint32_t buf = 0, use = 0;
+        for (int t = my_tile; t < p.tiles && ok; t += step) {
             const int n = t % p.tiles_n * ROWS + ew * 32 + lane, m0 = t / p.tiles_n * p.tile_m, rows = min(p.tile_m, p.M - m0);
-            ok &= mbar_wait(smem_u32(&tfull_bar[buf]), use & 1, &gave_up);
+            ok &= mbar_wait<LONG_WAIT>(smem_u32(&tfull_bar[buf]), use & 1, &gave_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem_base + buf * ACC_COLS + ((uint32_t)(ew * 32) << 16);
+            const uint32_t src = tmem_base + buf * 128 + ((uint32_t)(ew * 32) << 16);
 #pragma unroll 1
             for (int c = 0; c < rows; c += 16) {
                 uint32_t r[16];
@@ -525,6 +606,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[buf]));
+            if (++buf == (uint32_t)accs) buf = 0, use++;
         }
     }
     __syncwarp();
@@ -535,7 +617,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
         const int n0 = my_tile % p.tiles_n * ROWS, m0 = my_tile / p.tiles_n * p.tile_m, rows = min(p.tile_m, p.M - m0);
         if (warp >= FIRST_EPILOGUE) {
             const int ew = warp & 3;
-            ok &= mbar_wait(smem_u32(&tfull_bar[0]), 0, &gave_up);   // on give-up the drain still runs on whatever tensor memory holds
+            ok &= mbar_wait<LONG_WAIT>(smem_u32(&tfull_bar[0]), 0, &gave_up);   // on give-up the drain still runs on whatever tensor memory holds
             ok = __all_sync(0xffffffffu, ok);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -548,8 +630,8 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
         }
         __syncwarp();
         cluster_sync_all();
-        for (int i = threadIdx.x; i < ((rows - split + splits - 1) / splits) * ROWS; i += TALL_THREADS) {
-            const int row = i % ROWS, c = i / ROWS * splits + split;
+        for (int i = threadIdx.x; i < ((rows - split + splits - 1) >> shift) * ROWS; i += TALL_THREADS) {
+            const int row = i % ROWS, c = (i / ROWS << shift) + split;
             if (n0 + row >= p.N) continue;
             const uint32_t at = smem_u32(&sums[c * ROWS + row]);
             float v = 0.0f;
@@ -580,65 +662,68 @@ const char* const WHO = "matmul_w4";
 
 template <class T, int NT, int FLUSH, bool ZEROS>
 int launch(const Args& p) {
-    CUtensorMap mw, mx;
-    const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
-    if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, X_BOX_K, p.M < 8 * NT ? p.M : 8 * NT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
-    constexpr auto kern = matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
-    constexpr int smem = smem_of<NT>();
-    if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
-    const int tiles_n = (p.N - 1) / ROWS + 1, slabs = (p.K - 1) / SLAB_K + 1;
-    const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / (8 * NT) + 1);
-    int splits = 1;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps two slabs
-    while (splits < 8 && tiles * splits * 2 <= 2 * basalt_k::sm_count() && slabs >= splits * 4) splits *= 2;
-    if (tiles * splits > INT32_MAX) return basalt_k::record_msg(1, WHO, "M * N is too large");
-    return basalt_k::launch_clusters(WHO, kern, (unsigned)(tiles * splits), THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c, p.ldc, p.M, p.N, p.K,
-                                     p.group, tiles_n, p.status);
+    using S = few::Tile<NT>;
+    constexpr auto kern = few::matmul_w4_few<T, NT, FLUSH, ZEROS>;
+    if (const int rc = basalt_k::allow_smem<kern>(WHO, S::SMEM)) return rc;
+    const int tiles_n = (p.N - 1) / ROWS + 1, blocks = (p.K - 1) / few::BLOCK_K + 1;
+    const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / S::TOKENS + 1);
+    int shift = 0;   // two CTAs fit an SM: split K while the tiles leave room and every warp keeps two blocks
+    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && blocks >= 8 << shift) shift++;
+    const few::Shape q = {(const uint8_t*)p.w, p.x, p.scales, p.zeros, p.c, p.ldw, p.ldx, p.ldc, p.M, p.N, p.K, p.group, (p.K - 1) / p.group + 1, shift};
+    // a launch takes 65535 tiles of rows of X at most
+    for (int m = 0; m < p.M; m += 65535 * S::TOKENS) {
+        few::Shape part = q;
+        part.x = (const T*)p.x + m * p.ldx, part.c = (T*)p.c + m * p.ldc, part.M = p.M - m < 65535 * S::TOKENS ? p.M - m : 65535 * S::TOKENS;
+        const dim3 grid(tiles_n << shift, (part.M - 1) / S::TOKENS + 1);
+        if (const int rc = basalt_k::launch_clusters(WHO, kern, grid, few::THREADS, S::SMEM, 1 << shift, p.stream, part)) return rc;
+    }
+    return 0;
 }
 
-template <class T, int NT, int FLUSH>
-int launch_zeros(const Args& p) { return p.zeros ? launch<T, NT, FLUSH, true>(p) : launch<T, NT, FLUSH, false>(p); }
-
-template <class T, int NT>
-int launch_flush(const Args& p) {
-    const int units = p.group / UNIT_K;
-    return units % 4 == 0 ? launch_zeros<T, NT, 4>(p) : units % 2 == 0 ? launch_zeros<T, NT, 2>(p) : launch_zeros<T, NT, 1>(p);
-}
-
-template <class T, bool ZEROS>
+template <class T, int FLUSH, bool ZEROS>
 int launch_tall(const Args& p) {
-    const int sms = basalt_k::sm_count(), slabs = (p.K - 1) / SLAB_K + 1;
-    tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0};
-    // The width of a tile: of the few counts of tiles over M that come near 256 columns each, the one whose rounds over the SMs
+    constexpr int RAW_BYTES = tall::PACKED_BYTES + SlabScales<T, FLUSH, ZEROS>::BYTES;
+    const int sms = basalt_k::sm_count(), slabs = (p.K - 1) / tall::SLAB_K + 1;
+    tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0, (p.K - 1) / p.group + 1, 0};
+    // The width of a tile: of the few counts of tiles over M that come near 256 columns each the one whose rounds over the SMs
     // cost least. A slab costs two clocks a column, and not less than the unpacking of its weights, about 112 columns' worth.
     int64_t best = INT64_MAX;
-    for (int tiles_m = (p.M - 1) / 256 + 1, tries = 0; tries < 4; tries++, tiles_m++) {
+    for (int tiles_m = (p.M - 1) / tall::MAX_M + 1, tries = 0; tries < 4; tries++, tiles_m++) {
         const int width = ((p.M - 1) / tiles_m + 16) / 16 * 16;
         const int64_t tiles = (int64_t)((p.M - 1) / width + 1) * q.tiles_n, cost = ((tiles - 1) / sms + 1) * (width > 112 ? width : 112);
         if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
         if (cost < best) best = cost, q.tile_m = width, q.tiles = (int)tiles;
     }
-    const int stage = tall::W_TILE + q.tile_m * tall::TILE_K * 2;
-    q.raws = q.tile_m > 192 ? 2 : tall::MAX_RAW;
-    q.stages = (tall::SMEM_MOST - 1024 - q.raws * tall::RAW_BYTES) / stage;
+    const int stage = q.tile_m * tall::TILE_K * 2;
+    q.raws = q.tile_m > 160 ? 2 : tall::MAX_RAW;
+    q.stages = (tall::SMEM_MOST - 1024 - q.raws * RAW_BYTES) / stage;
     if (q.stages > tall::MAX_STAGES) q.stages = tall::MAX_STAGES;
-    const int smem = 1024 + q.raws * tall::RAW_BYTES + q.stages * stage;
-    int splits = 1;
-    while (splits < 8 && q.tiles * splits * 2 <= sms && slabs >= splits * 4) splits *= 2;
+    const int smem = 1024 + q.raws * RAW_BYTES + q.stages * stage;
+    while (q.split_shift < 3 && q.tiles << (q.split_shift + 1) <= sms && slabs >= 4 << q.split_shift) q.split_shift++;
+    const int splits = 1 << q.split_shift;
     CUtensorMap mw, mx;
     const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, SLAB_K / 2, ROWS)) return rc;
+    if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, tall::SLAB_K / 2, ROWS)) return rc;
     if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, tall::TILE_K, q.tile_m)) return rc;
-    constexpr auto kern = tall::matmul_w4_tall<T, ZEROS>;
+    constexpr auto kern = tall::matmul_w4_tall<T, FLUSH, ZEROS>;
     if (const int rc = basalt_k::allow_smem<kern>(WHO, tall::SMEM_MOST)) return rc;
     return basalt_k::launch_clusters(WHO, kern, splits > 1 || q.tiles < sms ? q.tiles * splits : sms, tall::TALL_THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales,
                                      p.zeros, (T*)p.c, p.ldc, q, p.status);
 }
 
+template <class T, int FLUSH, bool ZEROS>
+int launch_rows(const Args& p) {
+    if (p.M > 32 && p.N >= ROWS) return launch_tall<T, FLUSH, ZEROS>(p);
+    return p.M <= 8 ? launch<T, 1, FLUSH, ZEROS>(p) : p.M <= 16 ? launch<T, 2, FLUSH, ZEROS>(p) : launch<T, 4, FLUSH, ZEROS>(p);
+}
+
+template <class T, int FLUSH>
+int launch_zeros(const Args& p) { return p.zeros ? launch_rows<T, FLUSH, true>(p) : launch_rows<T, FLUSH, false>(p); }
+
 template <class T>
 int launch_type(const Args& p) {
-    if (p.M > 16 && p.N >= ROWS) return p.zeros ? launch_tall<T, true>(p) : launch_tall<T, false>(p);
-    return p.M <= 8 ? launch_flush<T, 1>(p) : launch_flush<T, 2>(p);
+    const int units = p.group / UNIT_K;
+    return units % 4 == 0 ? launch_zeros<T, 4>(p) : units % 2 == 0 ? launch_zeros<T, 2>(p) : launch_zeros<T, 1>(p);
 }
 
 }  // namespace
@@ -655,7 +740,8 @@ extern "C" int basalt_k_matmul_w4(int type, const void* X, int64_t ldx, const vo
     if (((uintptr_t)X | (uintptr_t)W) & 15 || ldw & 15 || ldx & 7) return basalt_k::record_msg(1, WHO, "X and W and their row strides must be multiples of 16 bytes");
     if (ldx < K || ldw < ((int64_t)K + 1) / 2 || ldc < N) return basalt_k::record_msg(1, WHO, "a row stride lies below the row");
     if (ldx >= (int64_t)1 << 31 || ldw >= (int64_t)1 << 31 || ldc >= (int64_t)1 << 31) return basalt_k::record_msg(1, WHO, "a row stride lies above 2^31 - 1");
-    if (((uintptr_t)C | (uintptr_t)scales) % 2 || (uintptr_t)status % 4) return basalt_k::record_msg(1, WHO, "C, the scales or the status are not aligned to their elements");
+    if (((uintptr_t)scales | (uintptr_t)zeros) % 4) return basalt_k::record_msg(1, WHO, "the scales and the zero points must start at a multiple of 4 bytes");
+    if ((uintptr_t)C % 2 || (uintptr_t)status % 4) return basalt_k::record_msg(1, WHO, "C or the status is not aligned to its elements");
     const int64_t groups = (K - 1) / group + 1, packed = ((int64_t)K + 1) / 2;
     const basalt_k::Span c = {C, M, N, ldc, 2};
     if (overlap(c, {X, M, K, ldx, 2}) || overlap(c, {W, N, packed, ldw, 1}) || overlap(c, {scales, N, groups, groups, 2}) || overlap(c, {zeros, N, groups, groups, 1}))
