@@ -489,30 +489,30 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             while (global_ns() - t0 < 2000000ull) {}
         }
     } else if (warp == WARP_MMA) {
-        // The warp stays together (see umma_f16_tmem): it shares its scheduler with warps that unpack, and every instruction waits its turn.
+        // The warp stays together (see umma_f16_tmem). It shares its scheduler with warps that unpack, every instruction waits its
+        // turn, and a tile of 64 k has at most 512 clocks: no vote on the waits (after one that gave up, the rest of the way
+        // is walked on whatever the memories hold), descriptors stepped by one addition a tile.
         const uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
         const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.tile_m >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-        const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]);
+        const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]), end = full0 + 8 * p.stages, w0 = tmem_base + WEIGHTS_AT;
         const uint64_t x0 = smem_desc(ring, 16, 1024), x_step = stage_bytes >> 4;
-        uint32_t s = 0, ph = 0, buf = 0, use = 0;
-        for (int t = my_tile; t < p.tiles && ok; t += step) {
+        uint32_t bar = full0, w = w0, ph = 0, buf = 0, use = 0;
+        uint64_t x = x0;
+        for (int t = my_tile; t < p.tiles; t += step) {
             ok &= mbar_wait(smem_u32(&tempty_bar[buf]), (use & 1) ^ 1, &gave_up);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t acc = tmem_base + buf * 128;
+            uint32_t accumulate = 0;
             for (int i = 0; i < count; i++) {
-                ok &= mbar_wait(full0 + 8 * s, ph, &gave_up);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                ok &= mbar_wait(bar, ph, &gave_up);
+                __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t w = tmem_base + WEIGHTS_AT + s * WEIGHT_COLS;
-                const uint64_t x = x0 + s * x_step;
-                umma_f16_tmem(acc, w, x, idesc, i != 0);
+                umma_f16_tmem(acc, w, x, idesc, accumulate);
+                accumulate = 1;
 #pragma unroll
                 for (int k = 1; k < TILE_K / 16; k++) umma_f16_tmem(acc, w + 8 * k, x + (uint64_t)(2 * k), idesc, 1);
-                umma_commit_elected(empty0 + 8 * s);
-                if (++s == (uint32_t)p.stages) s = 0, ph ^= 1;
+                umma_commit_elected(bar - full0 + empty0);
+                bar += 8, w += WEIGHT_COLS, x += x_step;
+                if (bar == end) bar = full0, w = w0, x = x0, ph ^= 1;
             }
             umma_commit_elected(smem_u32(&tfull_bar[buf]));
             if (++buf == (uint32_t)accs) buf = 0, use++;
