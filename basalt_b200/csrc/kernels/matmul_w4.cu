@@ -150,185 +150,150 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 
 // ---- few rows of X ----
 //
-// A CTA takes 128 rows of the weights over its share of K, in blocks of 128 k: four groups of 32 rows, the even and the odd blocks by
-// a warp each. A warp loads its weights from global memory straight into the registers it unpacks, 64 bytes of 32 rows a block,
-// and keeps DEEP blocks in flight; nothing but X goes through shared memory, where it lies in the order in which the
-// instructions want it, and no barrier stands in the loop.
-// (Through a ring of bulk loads the same sums took 12.7 us where this takes TIME_HERE, 8192 x 8192 for one row: the barriers and
-// addresses of each slab cost a third of its instructions.)
+// A CTA takes 128 rows of the weights over its share of K: one warp feeds a ring of stages (256 k) by bulk-tensor loads, eight
+// warps compute, 32 rows x half a stage each.
 namespace few {
-constexpr int BLOCK_K = 128, WARPS = 8, THREADS = 32 * WARPS, X_BYTES = 64 * 1024;
+constexpr int SLAB_K = 256, W_BYTES = ROWS * SLAB_K / 2, CONSUMERS = 8, THREADS = 32 * (CONSUMERS + 1), X_BOX_K = 32;
 
 template <int NT>
-struct Tile {
-    static constexpr int TOKENS = 8 * NT, DEEP = NT == 1 ? 3 : 2, JOIN = 2 * TOKENS * ROWS * 4;
-    static constexpr int ROUND = 2 * DEEP;   // blocks in which both warps have gone once through their registers' DEEP places
-    static constexpr int X_BLOCKS = X_BYTES / (TOKENS * BLOCK_K * 2) / ROUND * ROUND;
-    static constexpr int SMEM = X_BYTES + JOIN;   // at most 96 KB: two CTAs fit an SM
-};
+__host__ __device__ constexpr int x_bytes_of() { return 8 * NT * SLAB_K * 2; }
+template <int NT>
+__host__ __device__ constexpr int stages_of() { return NT == 1 ? 5 : 3; }
+template <int NT>
+__host__ __device__ constexpr int join_bytes_of() { return 2 * 8 * NT * ROWS * 4; }   // the sums of both halves of the warps, for every row of X
+template <int NT>
+__host__ __device__ constexpr int smem_of() { return stages_of<NT>() * (W_BYTES + x_bytes_of<NT>()) + join_bytes_of<NT>() + 1024; }   // at most 109 KB: two CTAs fit an SM
 
-// Where lane t of four finds word j of its weights in a block, in 8-k words: FLUSH words of the four lanes together hold k's that
-// certainly share a group (FLUSH * 32 of them).
-template <int FLUSH>
-__device__ __forceinline__ constexpr int word_of(int t, int j) { return FLUSH == 4 ? 4 * t + j : FLUSH == 2 ? 8 * (j >> 1) + 2 * t + (j & 1) : 4 * j + t; }
-
-template <class T, int FLUSH, bool ZEROS>
-struct Block {
-    uint32_t w[4][4];   // [row g + 8 r][word]
-    T scale[4 / FLUSH];
-    uint8_t zero[4 / FLUSH];
-};
-
-// `valid` bytes of four words; what lies behind is not read.
-__device__ __noinline__ uint32_t partial_word(const uint8_t* p, int valid) {
-    uint32_t v = 0;
-    for (int i = 0; i < valid && i < 4; i++) v |= (uint32_t)p[i] << (8 * i);
-    return v;
-}
-__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-struct Shape {
-    const uint8_t* w;
-    const void *x, *scales;
-    const uint8_t* zeros;
-    void* c;
-    int64_t ldw, ldx, ldc;
-    int M, N, K, group, groups, split_shift;   // a tile's K is shared by 1 << split_shift CTAs
-};
-
+// NT: tiles of eight rows of X. FLUSH: units (32 k) that certainly share a group, 1, 2 or 4.
 template <class T, int NT, int FLUSH, bool ZEROS>
-__global__ void __launch_bounds__(THREADS, 2) matmul_w4_few(const Shape p) {
-    using S = Tile<NT>;
-    constexpr int TOKENS = S::TOKENS, DEEP = S::DEEP, FLUSHES = 4 / FLUSH;
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
-    // (No division of the prologue is done that the host can do: on the way to the first load their latencies add up.)
-    const int shift = p.split_shift, splits = 1 << shift, split = blockIdx.x & (splits - 1), groups = p.groups, row_bytes = (p.K + 1) / 2;
-    const int n0 = (blockIdx.x >> shift) * ROWS, m0 = blockIdx.y * TOKENS, tokens = min(TOKENS, p.M - m0);
-    const int blocks = (p.K - 1) / BLOCK_K + 1, first = blocks * split >> shift, last = blocks * (split + 1) >> shift;
+__global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                               const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C, int64_t ldc,
+                                                               int M, int N, int K, int group, int groups, int shift, int32_t* status) {
+    constexpr int STAGES = stages_of<NT>(), TOKENS = 8 * NT, STAGE_BYTES = W_BYTES + x_bytes_of<NT>();
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
+    __shared__ volatile uint32_t gave_up;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (ring - smem_u32(smem_raw));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // 1 << shift CTAs share a tile's K. (No division is done here that the host can do: on the way to the first load their latencies add up.)
+    const int splits = 1 << shift, split = blockIdx.x & (splits - 1), n0 = (blockIdx.x >> shift) * ROWS, m0 = blockIdx.y * TOKENS;
+    const int slabs = (K - 1) / SLAB_K + 1, first = slabs * split >> shift, count = (slabs * (split + 1) >> shift) - first;
+
+    if (threadIdx.x == 0) {
+        prefetch_map(&map_w);
+        prefetch_map(&map_x);
+        gave_up = 0;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), CONSUMERS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
     cluster_arrive();
     wait_for_predecessor();
-
-    const uint8_t* w_row[4];   // this lane's part of rows g, g + 8, g + 16 and g + 24; rows past the last are computed with its weights, and not stored
-#pragma unroll
-    for (int r = 0; r < 4; r++) w_row[r] = p.w + (int64_t)min(n0 + row0 + g + 8 * r, p.N - 1) * p.ldw + 4 * word_of<FLUSH>(t, 0);
-    // Of those four rows, which four lanes share, lane t loads the scales of row g + 8 t, and the lanes exchange them.
-    const int64_t my_row = (int64_t)min(n0 + row0 + g + 8 * t, p.N - 1) * groups;
-    const T* scale_row = (const T*)p.scales + my_row;
-    const uint8_t* zero_row = ZEROS ? p.zeros + my_row : nullptr;
-    int which[FLUSHES], in_group[FLUSHES];   // the groups of the next block to load, and where in them its parts begin
-    which[0] = (unsigned)((first + half) * BLOCK_K) / (unsigned)p.group, in_group[0] = (first + half) * BLOCK_K - which[0] * p.group;
-#pragma unroll
-    for (int f = 1; f < FLUSHES; f++) {
-        which[f] = which[f - 1], in_group[f] = in_group[f - 1] + FLUSH * UNIT_K;
-        if (in_group[f] >= p.group) in_group[f] -= p.group, which[f]++;
-    }
-    const auto load = [&](Block<T, FLUSH, ZEROS>& b, int block) {
-        if (block >= last) return;
-        const int at = block * (BLOCK_K / 2);
-        if (at + BLOCK_K / 2 <= row_bytes) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint8_t* q = w_row[r] + at;
-                if constexpr (FLUSH == 4) {
-                    const uint4 v = load_stream(q);
-                    b.w[r][0] = v.x, b.w[r][1] = v.y, b.w[r][2] = v.z, b.w[r][3] = v.w;
-                } else if constexpr (FLUSH == 2) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(q)), u = __ldg(reinterpret_cast<const uint2*>(q + 32));
-                    b.w[r][0] = v.x, b.w[r][1] = v.y, b.w[r][2] = u.x, b.w[r][3] = u.y;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) b.w[r][j] = __ldg(reinterpret_cast<const uint32_t*>(q + 16 * j));
-                }
-            }
-        } else {   // the block in which the rows end
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int ahead = 4 * (word_of<FLUSH>(t, j) - word_of<FLUSH>(t, 0));
-                    b.w[r][j] = partial_word(w_row[r] + at + ahead, row_bytes - at - 4 * word_of<FLUSH>(t, j));
-                }
-        }
-#pragma unroll
-        for (int f = 0; f < FLUSHES; f++) {
-            const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
-            b.scale[f] = in ? scale_row[which[f]] : T(0.0f);
-            if (ZEROS) b.zero[f] = in ? zero_row[which[f]] : 0;
-            for (in_group[f] += 2 * BLOCK_K; in_group[f] >= p.group; in_group[f] -= p.group) which[f]++;
-        }
-    };
-
+    if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
+    bool ok = true;
     float total[2][NT][4] = {};
-    const auto compute = [&](const Block<T, FLUSH, ZEROS>& b, int block_here) {
-        const uint8_t* x_at = smem + block_here * (4 * TOKENS * 64) + lane * 16;
+
+    if (warp == CONSUMERS) {
+        if (lane == 0) {
+            for (int i = 0; i < count; i++) {
+                const int s = i % STAGES;
+                ok &= mbar_wait<LONG_WAIT>(smem_u32(&empty_bar[s]), ((i / STAGES) & 1) ^ 1, &gave_up);
+                if (!ok) break;
+                const uint32_t fb = smem_u32(&full_bar[s]), w_dst = ring + s * STAGE_BYTES, x_dst = w_dst + W_BYTES;
+                const int k = (first + i) * SLAB_K;
+                mbar_expect_tx(fb, W_BYTES + min(M, TOKENS) * SLAB_K * 2);
+                tma_load_2d(w_dst, &map_w, fb, k / 2, n0);
 #pragma unroll
-        for (int f = 0; f < FLUSHES; f++) {
-            Zero<T> z, row_z[4];
-            z.set(ZEROS ? b.zero[f] : 8);
+                for (int b = 0; b < SLAB_K / X_BOX_K; b++) tma_load_2d(x_dst + b * TOKENS * X_BOX_K * 2, &map_x, fb, k + b * X_BOX_K, m0);
+            }
+            if (!ok) {   // let the copies already issued land before the CTA can exit
+                const uint64_t t0 = global_ns();
+                while (global_ns() - t0 < 2000000ull) {}
+            }
+        }
+        __syncwarp();
+    } else {
+        const int half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
+        // Of the four weight rows g, g + 8, g + 16 and g + 24 that four lanes share, lane t loads the scales of row g + 8 t and the
+        // lanes exchange them. Those of a slab are loaded while the slab before is computed.
+        const int64_t n = min(n0 + row0 + g + 8 * t, N - 1);   // rows past the last are computed with its scales, and not stored
+        const T* scale_row = scales + n * groups;
+        const uint8_t* zero_row = ZEROS ? zeros + n * groups : nullptr;
+        T scale[4 / FLUSH];
+        uint8_t zero[4 / FLUSH];
+        int which[4 / FLUSH], in_group[4 / FLUSH];
+        auto load_scales = [&]() {
 #pragma unroll
-            for (int r = 0; r < 4; r++) row_z[r] = ZEROS ? z.of_lane((lane & ~3) | r) : z;
-            float acc[2][NT][4] = {};
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
+                scale[f] = in ? scale_row[which[f]] : T(0.0f);
+                if (ZEROS) zero[f] = in ? zero_row[which[f]] : 0;
+                for (in_group[f] += SLAB_K; in_group[f] >= group; in_group[f] -= group) which[f]++;
+            }
+        };
+        which[0] = (unsigned)(first * SLAB_K + half * 128) / (unsigned)group, in_group[0] = first * SLAB_K + half * 128 - which[0] * group;
 #pragma unroll
-            for (int v = 0; v < FLUSH; v++) {
-                const int j = f * FLUSH + v;
-                uint32_t a[4][4];
+        for (int f = 1; f < 4 / FLUSH; f++) {
+            which[f] = which[f - 1], in_group[f] = in_group[f - 1] + FLUSH * UNIT_K;
+            if (in_group[f] >= group) in_group[f] -= group, which[f]++;
+        }
+        load_scales();
+        for (int i = 0; i < count; i++) {
+            const int s = i % STAGES;
+            float by[4 / FLUSH];
+            Zero<T> z[ZEROS ? 4 / FLUSH : 1];
+            if (!ZEROS) z[0].set(8);
 #pragma unroll
-                for (int r = 0; r < 4; r++) unpack(b.w[r][j], row_z[r], a[r]);
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                by[f] = to_float(scale[f]);
+                if (ZEROS) z[f].set(zero[f]);
+            }
+            load_scales();
+            ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint8_t* w_at = smem + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
+            const uint8_t* x_at = smem + s * STAGE_BYTES + W_BYTES + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(x_at + (j * TOKENS + 8 * nt) * 64);   // row 8 nt + g of X, the k's of word j of lane t
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                float acc[2][NT][4] = {};
+                Zero<T> row_z[4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        mma_16816<T>(acc[h][nt], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
-                        mma_16816<T>(acc[h][nt], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x.z, x.w);
+                for (int r = 0; r < 4; r++) row_z[r] = ZEROS ? z[ZEROS ? f : 0].of_lane((lane & ~3) | r) : z[0];
+#pragma unroll
+                for (int v = 0; v < FLUSH; v++) {
+                    const int u = f * FLUSH + v;
+                    uint32_t a[4][4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) unpack(*reinterpret_cast<const uint32_t*>(w_at + r * 8 * 128 + (((half * 4 + u) ^ g) << 4)), row_z[r], a[r]);   // 128-byte swizzle: piece ^ (row & 7)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(x_at + u * TOKENS * X_BOX_K * 2 + nt * 8 * X_BOX_K * 2);   // row 8 nt + g of X, its k 8 t .. 8 t + 7 of the unit
+                        const uint32_t b0 = __byte_perm(x.x, x.z, 0x5410), b1 = __byte_perm(x.x, x.z, 0x7632);
+                        const uint32_t b2 = __byte_perm(x.y, x.w, 0x5410), b3 = __byte_perm(x.y, x.w, 0x7632);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            mma_16816<T>(acc[h][nt], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], b0, b1);
+                            mma_16816<T>(acc[h][nt], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], b2, b3);
+                        }
                     }
                 }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float b = __shfl_sync(0xffffffffu, by[f], (lane & ~3) | r);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) total[r >> 1][nt][2 * (r & 1) + j] += b * acc[r >> 1][nt][2 * (r & 1) + j];
+                }
             }
-            const float my_scale = to_float(b.scale[f]);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float row_scale = __shfl_sync(0xffffffffu, my_scale, (lane & ~3) | r);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) total[r >> 1][nt][2 * (r & 1) + j] += row_scale * acc[r >> 1][nt][2 * (r & 1) + j];
-            }
-        }
-    };
-
-    Block<T, FLUSH, ZEROS> b[DEEP];
-#pragma unroll
-    for (int d = 0; d < DEEP; d++) load(b[d], first + half + 2 * d);
-    for (int from = first; from < last; from += S::X_BLOCKS) {   // as many blocks of X as shared memory takes
-        const int to = min(from + S::X_BLOCKS, last), pieces = (to - from) * (BLOCK_K / 8);
-        if (from != first) __syncthreads();   // the blocks before have been computed
-        for (int m = 0; m < tokens; m++)
-        for (int q = threadIdx.x; q < pieces; q += THREADS) {   // eight k of a row of X each, in the order of the pairs that unpack() makes
-            const int word = q % 16, k = from * BLOCK_K + q * 8;
-            const T* x = (const T*)p.x + (m0 + m) * p.ldx + k;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (k + 8 <= p.K) v = __ldg(reinterpret_cast<const uint4*>(x));
-            else if (k < p.K) {
-                uint32_t e[4] = {0, 0, 0, 0};
-                for (int c = 0; c < p.K - k; c++) e[c / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(x)[c] << (16 * (c % 2));
-                v = make_uint4(e[0], e[1], e[2], e[3]);
-            }
-            const int wt = FLUSH == 4 ? word >> 2 : FLUSH == 2 ? (word & 7) >> 1 : word & 3, wj = FLUSH == 4 ? word & 3 : FLUSH == 2 ? (word >> 3) * 2 + (word & 1) : word >> 2;
-            *reinterpret_cast<uint4*>(smem + (((q / 16) * 4 + wj) * TOKENS + m) * 64 + wt * 16) =
-                make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        }
-        __syncthreads();
-        for (int block = from + half; block < to; block += 2 * DEEP) {
-#pragma unroll
-            for (int d = 0; d < DEEP; d++) {
-                if (block + 2 * d < to) compute(b[d], block + 2 * d - from);
-                if (block + 2 * d < to) load(b[d], block + 2 * (d + DEEP));
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
         }
     }
 
@@ -336,28 +301,31 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_few(const Shape p) {
     // warp stores its sums where that CTA will read them.
     __syncwarp();
     cluster_wait();   // every CTA of the cluster runs, so its shared memory is there
-    const int each = TOKENS >> shift;
-    float* join = reinterpret_cast<float*>(smem + X_BYTES);   // [CTA][half][row of X, of those this CTA adds up][row of the weights]
-    const uint32_t mine = smem_u32(join + (split * 2 + half) * each * ROWS + row0 + g);
+    const int tokens = min(TOKENS, M - m0), each = TOKENS >> shift;
+    float* join = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);   // [CTA][half][row of X, of those this CTA adds up][row of the weights]
+    if (warp < CONSUMERS) {
+        const uint32_t mine = smem_u32(join + (split * 2 + (warp >> 2)) * each * ROWS + (warp & 3) * 32 + (lane >> 2));
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int c = 8 * nt + 2 * t + e;
-            if (c >= tokens) continue;
-            const uint32_t to = map_to_cta(mine + (c >> shift) * ROWS * 4, c & (splits - 1));
+            for (int e = 0; e < 2; e++) {
+                const int c = 8 * nt + 2 * (lane & 3) + e;
+                if (c >= tokens) continue;
+                const uint32_t to = map_to_cta(mine + (c >> shift) * ROWS * 4, c & (splits - 1));
 #pragma unroll
-            for (int r = 0; r < 4; r++) store_cluster_f32(to + 8 * r * 4, total[r >> 1][nt][2 * (r & 1) + e]);
-        }
+                for (int r = 0; r < 4; r++) store_cluster_f32(to + 8 * r * 4, total[r >> 1][nt][2 * (r & 1) + e]);
+            }
+    }
     __syncwarp();
     cluster_sync_all();
     for (int i = threadIdx.x; i < ((tokens - split + splits - 1) >> shift) * ROWS; i += THREADS) {
         const int row = i % ROWS, c = (i / ROWS << shift) + split;
-        if (n0 + row >= p.N) continue;
+        if (n0 + row >= N) continue;
         float v = 0.0f;
         for (int q = 0; q < 2 * splits; q++) v += join[(q * each + i / ROWS) * ROWS + row];
-        store_as((T*)p.c + (m0 + c) * p.ldc + n0 + row, v);
+        store_as(C + (m0 + c) * ldc + n0 + row, v);
     }
+    if (!ok && status) atomicExch(status, 1);
 }
 }  // namespace few
 
@@ -660,22 +628,29 @@ struct Args {
 
 const char* const WHO = "matmul_w4";
 
+template <class T>
+constexpr CUtensorMapDataType MAP_TYPE = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+
 template <class T, int NT, int FLUSH, bool ZEROS>
-int launch(const Args& p) {
-    using S = few::Tile<NT>;
-    constexpr auto kern = few::matmul_w4_few<T, NT, FLUSH, ZEROS>;
-    if (const int rc = basalt_k::allow_smem<kern>(WHO, S::SMEM)) return rc;
-    const int tiles_n = (p.N - 1) / ROWS + 1, blocks = (p.K - 1) / few::BLOCK_K + 1;
-    const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / S::TOKENS + 1);
-    int shift = 0;   // two CTAs fit an SM: split K while the tiles leave room and every warp keeps two blocks
-    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && blocks >= 8 << shift) shift++;
-    const few::Shape q = {(const uint8_t*)p.w, p.x, p.scales, p.zeros, p.c, p.ldw, p.ldx, p.ldc, p.M, p.N, p.K, p.group, (p.K - 1) / p.group + 1, shift};
-    // a launch takes 65535 tiles of rows of X at most
-    for (int m = 0; m < p.M; m += 65535 * S::TOKENS) {
-        few::Shape part = q;
-        part.x = (const T*)p.x + m * p.ldx, part.c = (T*)p.c + m * p.ldc, part.M = p.M - m < 65535 * S::TOKENS ? p.M - m : 65535 * S::TOKENS;
-        const dim3 grid(tiles_n << shift, (part.M - 1) / S::TOKENS + 1);
-        if (const int rc = basalt_k::launch_clusters(WHO, kern, grid, few::THREADS, S::SMEM, 1 << shift, p.stream, part)) return rc;
+int launch_few(const Args& p) {
+    constexpr int TOKENS = 8 * NT, smem = few::smem_of<NT>();
+    constexpr auto kern = few::matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
+    if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
+    const int tiles_n = (p.N - 1) / ROWS + 1, slabs = (p.K - 1) / few::SLAB_K + 1, groups = (p.K - 1) / p.group + 1;
+    const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TOKENS + 1);
+    int shift = 0;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps two slabs
+    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && slabs >= 4 << shift) shift++;
+    CUtensorMap mw, mx;
+    if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, few::SLAB_K / 2, ROWS)) return rc;
+    // one launch takes 65535 tiles of rows of X
+    for (int m = 0; m < p.M; m += 65535 * TOKENS) {
+        const int rows = p.M - m < 65535 * TOKENS ? p.M - m : 65535 * TOKENS;
+        if (const int rc = make_tensor_map(&mx, WHO, MAP_TYPE<T>, (const T*)p.x + m * p.ldx, rows, p.K, p.ldx * 2, few::X_BOX_K, rows < TOKENS ? rows : TOKENS, CU_TENSOR_MAP_SWIZZLE_NONE))
+            return rc;
+        const dim3 grid(tiles_n << shift, (rows - 1) / TOKENS + 1);
+        if (const int rc = basalt_k::launch_clusters(WHO, kern, grid, few::THREADS, smem, 1 << shift, p.stream, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c + m * p.ldc, p.ldc, rows,
+                                                     p.N, p.K, p.group, groups, shift, p.status))
+            return rc;
     }
     return 0;
 }
@@ -702,9 +677,8 @@ int launch_tall(const Args& p) {
     while (q.split_shift < 3 && q.tiles << (q.split_shift + 1) <= sms && slabs >= 4 << q.split_shift) q.split_shift++;
     const int splits = 1 << q.split_shift;
     CUtensorMap mw, mx;
-    const auto x_type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, tall::SLAB_K / 2, ROWS)) return rc;
-    if (const int rc = make_tensor_map(&mx, WHO, x_type, p.x, p.M, p.K, p.ldx * 2, tall::TILE_K, q.tile_m)) return rc;
+    if (const int rc = make_tensor_map(&mx, WHO, MAP_TYPE<T>, p.x, p.M, p.K, p.ldx * 2, tall::TILE_K, q.tile_m)) return rc;
     constexpr auto kern = tall::matmul_w4_tall<T, FLUSH, ZEROS>;
     if (const int rc = basalt_k::allow_smem<kern>(WHO, tall::SMEM_MOST)) return rc;
     return basalt_k::launch_clusters(WHO, kern, splits > 1 || q.tiles < sms ? q.tiles * splits : sms, tall::TALL_THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales,
@@ -713,8 +687,8 @@ int launch_tall(const Args& p) {
 
 template <class T, int FLUSH, bool ZEROS>
 int launch_rows(const Args& p) {
-    if (p.M > 32 && p.N >= ROWS) return launch_tall<T, FLUSH, ZEROS>(p);
-    return p.M <= 8 ? launch<T, 1, FLUSH, ZEROS>(p) : p.M <= 16 ? launch<T, 2, FLUSH, ZEROS>(p) : launch<T, 4, FLUSH, ZEROS>(p);
+    if (p.M > 16 && p.N >= ROWS) return launch_tall<T, FLUSH, ZEROS>(p);
+    return p.M <= 8 ? launch_few<T, 1, FLUSH, ZEROS>(p) : launch_few<T, 2, FLUSH, ZEROS>(p);
 }
 
 template <class T, int FLUSH>

@@ -285,8 +285,8 @@ def test_matmul_w4_random(gpu, shape, t):
     q, s, z, w = w4_weights(g, N, K, group, M != 1, t, False)
     want, size = x.double() @ w.T, x.double().abs() @ w.abs().T
     got = run_w4(gpu, x, q, s, z, group, t, 0).double()
-    # beyond 32 rows a weight may be rounded to X's type before the product: half a step of |w| each
-    weight = HALF[t] if M > 32 else 0.0
+    # beyond 16 rows a weight may be rounded to X's type before the product: half a step of |w| each
+    weight = HALF[t] if M > 16 else 0.0
     assert ((got - want).abs() <= want.abs() * (HALF[t] * (1 + 2 ** -7) + 2 * U) + size * (2 * K * U + weight) + TINY[t]).all()
 
 
@@ -348,7 +348,7 @@ def test_a_layer_of_them(gpu, rows_n):
     assert ((got["y"].double() - y).abs() <= y.abs() * (half * (1 + 2 ** -7) + rel)).all()
     x = got["y"].double()
     want, size = x @ w4.T, x.abs() @ w4.abs().T
-    weight = half if rows_n > 32 else 0.0
+    weight = half if rows_n > 16 else 0.0
     assert ((got["c4"].double() - want).abs() <= want.abs() * (half * (1 + 2 ** -7) + 2 * U) + size * (2 * hidden * U + weight)).all()
 
 
