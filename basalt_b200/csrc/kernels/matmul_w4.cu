@@ -32,46 +32,85 @@ using namespace basalt_k::tc;
 
 constexpr int ROWS = 128, UNIT_K = 32;
 
+template <class T>
+__device__ __forceinline__ T as_type(uint32_t bits) {
+    if constexpr (std::is_same_v<T, __half>) return __ushort_as_half((unsigned short)bits);
+    else return __ushort_as_bfloat16((unsigned short)bits);
+}
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// The 4-byte word at `offset` of `from` to shared memory, asynchronously; what lies behind `end` is not read, and arrives as zeros.
-__device__ __forceinline__ void copy_word(uint32_t to, const void* from, int64_t offset, int64_t end) {
-    const int bytes = (int)max((int64_t)0, min((int64_t)4, end - offset));
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"((const uint8_t*)from + (bytes ? offset : 0)), "r"(bytes) : "memory");
+// BYTES (4, 8 or 16, and so aligned) from global to shared memory, asynchronously. The first `valid` of them are read (none, if it is
+// negative); the others arrive as zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, int valid = BYTES) {
+    const int n = max(0, min(BYTES, valid));
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
 }
 // Arrives on the barrier when every copy that this thread has begun is done.
 __device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory"); }
 
 // A slab's scales and zero points in shared memory: of each of the tile's 128 rows the groups that 256 k touch, at most 8 / FLUSH where
-// FLUSH * 32 k certainly share a group, as the 4-byte words that hold them. (A load by each thread that wants a scale
-// touches 32 rows, so 32 lines of the cache, in an instruction: with those the unpacking of 64 k took 900 clocks, SCALES_HERE with this.)
+// FLUSH * 32 k certainly share a group. They travel with the slab's weights. (A load by each thread that wants a scale touches 32
+// rows, so 32 lines of the cache, in an instruction: with those, one row through 8192 x 8192 in groups of 32 took 34 us.)
+// ALIGNED: every slab begins with a group and its groups are whole pieces of 4, 8 or 16 bytes; else as many 4-byte words as hold
+// them from any start.
 template <class T, int FLUSH, bool ZEROS>
 struct SlabScales {
-    static constexpr int GROUPS = 8 / FLUSH, SCALE_WORDS = GROUPS / 2 + 1, ZERO_WORDS = ZEROS ? (GROUPS + 6) / 4 : 0;
+    static constexpr int GROUPS = 8 / FLUSH, SCALE_WORDS = GROUPS / 2 + 1, ZERO_WORDS = ZEROS ? (GROUPS + 6) / 4 : 0, ZERO_PIECE = GROUPS < 4 ? 4 : GROUPS;
     static constexpr int ZERO_AT = ROWS * SCALE_WORDS * 4, BYTES = (ZERO_AT + ROWS * ZERO_WORDS * 4 + 1023) / 1024 * 1024;
 
-    // One warp's copies for the rows from n0, beginning with group `start`; `at`: where in shared memory.
-    static __device__ __forceinline__ void copy(uint32_t at, const void* scales, const void* zeros, int n0, int N, int groups, int start, int lane) {
-        const int64_t scale_end = (int64_t)N * groups * 2, zero_end = (int64_t)N * groups;
+    static bool aligned(const void* scales, const void* zeros, int group, int groups) {
+        return group * GROUPS == 256 && groups % GROUPS == 0 && (uintptr_t)scales % (2 * GROUPS) == 0 && (uintptr_t)zeros % ZERO_PIECE == 0;
+    }
+
+    // One warp's copies of the rows from n0; lane l has rows l, l + 32, l + 64 and l + 96.
+    struct Copies {
+        const uint8_t *scale_row[4], *zero_row[4], *scale_end, *zero_end;
+        __device__ __forceinline__ Copies(const void* scales, const uint8_t* zeros, int n0, int N, int groups, int lane) {
+            scale_end = (const uint8_t*)scales + (int64_t)N * groups * 2, zero_end = zeros + (ZEROS ? (int64_t)N * groups : 0);
 #pragma unroll
-        for (int r = 0; r < ROWS / 32; r++) {
-            const int row = lane + 32 * r;
-            const int64_t group = (int64_t)min(n0 + row, N - 1) * groups + start;   // rows past the last get its scales
-#pragma unroll
-            for (int w = 0; w < SCALE_WORDS; w++) copy_word(at + (row * SCALE_WORDS + w) * 4, scales, (group * 2 & ~3LL) + 4 * w, scale_end);
-#pragma unroll
-            for (int w = 0; w < ZERO_WORDS; w++) copy_word(at + ZERO_AT + (row * ZERO_WORDS + w) * 4, zeros, (group & ~3LL) + 4 * w, zero_end);
+            for (int r = 0; r < 4; r++) {
+                const int64_t first = (int64_t)min(n0 + lane + 32 * r, N - 1) * groups;   // rows past the last get its scales
+                scale_row[r] = (const uint8_t*)scales + first * 2, zero_row[r] = zeros + (ZEROS ? first : 0);
+            }
         }
+        // those of the groups from `start`, to `at` in shared memory
+        __device__ __forceinline__ void operator()(uint32_t at, int start, int lane, bool aligned) const {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = lane + 32 * r;
+                const uint8_t *s = scale_row[r] + 2 * start, *z = zero_row[r] + start;
+                if (aligned) {
+                    copy_async<2 * GROUPS>(at + row * 2 * GROUPS, s);
+                    if (ZEROS) {
+                        const uint8_t* piece = (const uint8_t*)((uintptr_t)z & ~(uintptr_t)(ZERO_PIECE - 1));
+                        copy_async<ZERO_PIECE>(at + ZERO_AT + row * ZERO_PIECE, piece, (int)min((int64_t)ZERO_PIECE, zero_end - piece));
+                    }
+                } else {
+                    const uint8_t *sw = (const uint8_t*)((uintptr_t)s & ~(uintptr_t)3), *zw = (const uint8_t*)((uintptr_t)z & ~(uintptr_t)3);
+#pragma unroll
+                    for (int w = 0; w < SCALE_WORDS; w++) {
+                        const bool in = sw + 4 * w < scale_end;
+                        copy_async<4>(at + (row * SCALE_WORDS + w) * 4, in ? sw + 4 * w : scale_row[0], in ? (int)min((int64_t)4, scale_end - sw - 4 * w) : 0);
+                    }
+#pragma unroll
+                    for (int w = 0; w < ZERO_WORDS; w++) {
+                        const bool in = zw + 4 * w < zero_end;
+                        copy_async<4>(at + ZERO_AT + (row * ZERO_WORDS + w) * 4, in ? zw + 4 * w : zero_row[0], in ? (int)min((int64_t)4, zero_end - zw - 4 * w) : 0);
+                    }
+                }
+            }
+        }
+    };
+    // The scale (its bits) and the zero point of row `row` in group start + ahead; row_group: the row's first group, modulo 4 at least.
+    static __device__ __forceinline__ uint32_t scale_bits(const uint8_t* at, int row, uint32_t row_group, int start, int ahead, bool aligned) {
+        return *reinterpret_cast<const uint16_t*>(at + (aligned ? row * 2 * GROUPS : row * SCALE_WORDS * 4 + ((row_group + start) & 1) * 2) + ahead * 2);
     }
-    // The scale and zero point of row `row` and group start + ahead; row_group: N row's first group, modulo 4 at least.
-    static __device__ __forceinline__ uint32_t scale_bits(const uint8_t* at, int row, uint32_t row_group, int start, int ahead) {
-        return reinterpret_cast<const uint16_t*>(at + row * SCALE_WORDS * 4)[((row_group + start) & 1) + ahead];
-    }
-    static __device__ __forceinline__ int zero(const uint8_t* at, int row, uint32_t row_group, int start, int ahead) {
-        return at[ZERO_AT + row * ZERO_WORDS * 4 + ((row_group + start) & 3) + ahead];
+    static __device__ __forceinline__ int zero(const uint8_t* at, int row, uint32_t row_group, int start, int ahead, bool aligned) {
+        return at[ZERO_AT + (aligned ? row * ZERO_PIECE + ((row_group + start) & (ZERO_PIECE - 1)) : row * ZERO_WORDS * 4 + ((row_group + start) & 3)) + ahead];
     }
 };
 
@@ -89,7 +128,7 @@ template <>
 struct Zero<__half> {
     __half2 low, high;
     __device__ __forceinline__ void set(int z) {
-        low = __half2half2(__int2half_rn(1024 + z));
+        low = __half2half2(__ushort_as_half((unsigned short)(0x6400 + z)));   // 1024 + z: z counts the last bits of the mantissa
         high = __hsub2(__half2half2(__int2half_rn(960)), low);   // -64 - z
     }
     __device__ __forceinline__ Zero of_lane(int lane) const {
@@ -102,7 +141,7 @@ struct Zero<__half> {
 template <>
 struct Zero<__nv_bfloat16> {
     __nv_bfloat162 low;
-    __device__ __forceinline__ void set(int z) { low = __bfloat162bfloat162(__int2bfloat16_rn(128 + z)); }
+    __device__ __forceinline__ void set(int z) { low = __bfloat162bfloat162(__ushort_as_bfloat16((unsigned short)(0x4300 + z))); }   // 128 + z, likewise
     __device__ __forceinline__ Zero of_lane(int lane) const {
         Zero v;
         v.low = __shfl_sync(0xffffffffu, low, lane);
@@ -155,21 +194,22 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 namespace few {
 constexpr int SLAB_K = 256, W_BYTES = ROWS * SLAB_K / 2, CONSUMERS = 8, THREADS = 32 * (CONSUMERS + 1), X_BOX_K = 32;
 
-template <int NT>
-__host__ __device__ constexpr int x_bytes_of() { return 8 * NT * SLAB_K * 2; }
-template <int NT>
-__host__ __device__ constexpr int stages_of() { return NT == 1 ? 5 : 3; }
-template <int NT>
-__host__ __device__ constexpr int join_bytes_of() { return 2 * 8 * NT * ROWS * 4; }   // the sums of both halves of the warps, for every row of X
-template <int NT>
-__host__ __device__ constexpr int smem_of() { return stages_of<NT>() * (W_BYTES + x_bytes_of<NT>()) + join_bytes_of<NT>() + 1024; }   // at most 109 KB: two CTAs fit an SM
+// A stage: 128 rows of weights, 8 NT rows of X, the scales. JOIN: the sums of both halves of the warps, for every row of X.
+template <class T, int NT, int FLUSH, bool ZEROS>
+struct Stage {
+    using Scales = SlabScales<T, FLUSH, ZEROS>;
+    static constexpr int X = W_BYTES, SCALES = X + 8 * NT * SLAB_K * 2, BYTES = SCALES + Scales::BYTES, COUNT = NT == 1 ? 4 : 3, JOIN = 2 * 8 * NT * ROWS * 4;
+    static constexpr int SMEM = COUNT * BYTES + JOIN + 1024;   // at most 109 KB: two CTAs fit an SM
+};
 
 // NT: tiles of eight rows of X. FLUSH: units (32 k) that certainly share a group, 1, 2 or 4.
 template <class T, int NT, int FLUSH, bool ZEROS>
 __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C, int64_t ldc,
-                                                               int M, int N, int K, int group, int groups, int shift, int32_t* status) {
-    constexpr int STAGES = stages_of<NT>(), TOKENS = 8 * NT, STAGE_BYTES = W_BYTES + x_bytes_of<NT>();
+                                                               int M, int N, int K, int group, int groups, int aligned, int shift, int32_t* status) {
+    using S = Stage<T, NT, FLUSH, ZEROS>;
+    using Scales = typename S::Scales;
+    constexpr int STAGES = S::COUNT, TOKENS = 8 * NT, STAGE_BYTES = S::BYTES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES];
     __shared__ volatile uint32_t gave_up;
@@ -185,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
         prefetch_map(&map_x);
         gave_up = 0;
         for (int s = 0; s < STAGES; s++) {
-            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&full_bar[s]), 1 + 32);   // the bulk loads, and each lane's copies of scales
             mbar_init(smem_u32(&empty_bar[s]), CONSUMERS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -198,67 +238,60 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
     bool ok = true;
     float total[2][NT][4] = {};
 
+    const int first_group = (unsigned)(first * SLAB_K) / (unsigned)group;
     if (warp == CONSUMERS) {
-        if (lane == 0) {
-            for (int i = 0; i < count; i++) {
-                const int s = i % STAGES;
-                ok &= mbar_wait<LONG_WAIT>(smem_u32(&empty_bar[s]), ((i / STAGES) & 1) ^ 1, &gave_up);
-                if (!ok) break;
-                const uint32_t fb = smem_u32(&full_bar[s]), w_dst = ring + s * STAGE_BYTES, x_dst = w_dst + W_BYTES;
-                const int k = (first + i) * SLAB_K;
+        const typename Scales::Copies copies(scales, zeros, n0, N, groups, lane);
+        int start = first_group, in_group = first * SLAB_K - start * group;
+        for (int i = 0; i < count; i++) {
+            const int s = i % STAGES;
+            ok &= mbar_wait<LONG_WAIT>(smem_u32(&empty_bar[s]), ((i / STAGES) & 1) ^ 1, &gave_up);
+            if (!ok) break;
+            const uint32_t fb = smem_u32(&full_bar[s]), at = ring + s * STAGE_BYTES;
+            const int k = (first + i) * SLAB_K;
+            if (lane == 0) {
                 mbar_expect_tx(fb, W_BYTES + min(M, TOKENS) * SLAB_K * 2);
-                tma_load_2d(w_dst, &map_w, fb, k / 2, n0);
+                tma_load_2d(at, &map_w, fb, k / 2, n0);
 #pragma unroll
-                for (int b = 0; b < SLAB_K / X_BOX_K; b++) tma_load_2d(x_dst + b * TOKENS * X_BOX_K * 2, &map_x, fb, k + b * X_BOX_K, m0);
+                for (int b = 0; b < SLAB_K / X_BOX_K; b++) tma_load_2d(at + S::X + b * TOKENS * X_BOX_K * 2, &map_x, fb, k + b * X_BOX_K, m0);
             }
-            if (!ok) {   // let the copies already issued land before the CTA can exit
-                const uint64_t t0 = global_ns();
-                while (global_ns() - t0 < 2000000ull) {}
-            }
+            copies(at + S::SCALES, start, lane, aligned);
+            copies_arrive(fb);
+            for (in_group += SLAB_K; in_group >= group; in_group -= group) start++;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok) {   // let the copies already issued land before the CTA can exit
+            const uint64_t t0 = global_ns();
+            while (global_ns() - t0 < 2000000ull) {}
         }
         __syncwarp();
     } else {
         const int half = warp >> 2, row0 = (warp & 3) * 32, g = lane >> 2, t = lane & 3;
-        // Of the four weight rows g, g + 8, g + 16 and g + 24 that four lanes share, lane t loads the scales of row g + 8 t and the
-        // lanes exchange them. Those of a slab are loaded while the slab before is computed.
-        const int64_t n = min(n0 + row0 + g + 8 * t, N - 1);   // rows past the last are computed with its scales, and not stored
-        const T* scale_row = scales + n * groups;
-        const uint8_t* zero_row = ZEROS ? zeros + n * groups : nullptr;
-        T scale[4 / FLUSH];
-        uint8_t zero[4 / FLUSH];
-        int which[4 / FLUSH], in_group[4 / FLUSH];
-        auto load_scales = [&]() {
-#pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++) {
-                const bool in = which[f] < groups;   // past the end of K: X is zero there, and so is the scale
-                scale[f] = in ? scale_row[which[f]] : T(0.0f);
-                if (ZEROS) zero[f] = in ? zero_row[which[f]] : 0;
-                for (in_group[f] += SLAB_K; in_group[f] >= group; in_group[f] -= group) which[f]++;
-            }
-        };
-        which[0] = (unsigned)(first * SLAB_K + half * 128) / (unsigned)group, in_group[0] = first * SLAB_K + half * 128 - which[0] * group;
-#pragma unroll
-        for (int f = 1; f < 4 / FLUSH; f++) {
-            which[f] = which[f - 1], in_group[f] = in_group[f - 1] + FLUSH * UNIT_K;
-            if (in_group[f] >= group) in_group[f] -= group, which[f]++;
-        }
-        load_scales();
+        // Of the four weight rows g, g + 8, g + 16 and g + 24 that four lanes share, lane t reads the scales of row g + 8 t and the
+        // lanes exchange them.
+        const int my_row = row0 + g + 8 * t;
+        const uint32_t row_group = (uint32_t)min(n0 + my_row, N - 1) * (uint32_t)groups;
+        int start = first_group, in_start = first * SLAB_K - start * group;
         for (int i = 0; i < count; i++) {
             const int s = i % STAGES;
-            float by[4 / FLUSH];
-            Zero<T> z[ZEROS ? 4 / FLUSH : 1];
-            if (!ZEROS) z[0].set(8);
-#pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++) {
-                by[f] = to_float(scale[f]);
-                if (ZEROS) z[f].set(zero[f]);
-            }
-            load_scales();
             ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            const uint8_t* my_scales = smem + s * STAGE_BYTES + S::SCALES;
+            float by[4 / FLUSH];
+            Zero<T> z[ZEROS ? 4 / FLUSH : 1];
+            if (!ZEROS) z[0].set(8);
+            int ahead = 0, k = in_start + half * 128;   // the group of this half's next part, counted from the slab's first
+#pragma unroll
+            for (int f = 0; f < 4 / FLUSH; f++) {
+                for (; k >= group; k -= group) ahead++;
+                const bool in = start + ahead < groups;   // past the end of K: X is zero there, and so is the scale
+                by[f] = in ? to_float(as_type<T>(Scales::scale_bits(my_scales, my_row, row_group, start, ahead, aligned))) : 0.0f;
+                if (ZEROS) z[f].set(in ? Scales::zero(my_scales, my_row, row_group, start, ahead, aligned) : 0);
+                k += FLUSH * UNIT_K;
+            }
+            for (in_start += SLAB_K; in_start >= group; in_start -= group) start++;
             const uint8_t* w_at = smem + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
-            const uint8_t* x_at = smem + s * STAGE_BYTES + W_BYTES + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
+            const uint8_t* x_at = smem + s * STAGE_BYTES + S::X + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
 #pragma unroll
             for (int f = 0; f < 4 / FLUSH; f++) {
                 float acc[2][NT][4] = {};
@@ -359,7 +392,7 @@ __device__ __forceinline__ void unpack_scaled(uint32_t w, uint32_t zero, uint32_
     }
 }
 struct Shape {
-    int M, N, K, group, tile_m, tiles_n, tiles, stages, raws, groups, split_shift;
+    int M, N, K, group, tile_m, tiles_n, tiles, stages, raws, groups, split_shift, aligned;
 };
 
 template <class T, int FLUSH, bool ZEROS>
@@ -436,6 +469,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
         uint32_t ph = 0;
         for (int t = my_tile; t < p.tiles && ok; t += step) {
             const int n0 = t % p.tiles_n * ROWS;
+            const typename Scales::Copies copies(scales, zeros, n0, p.N, p.groups, lane);
             int start = first_group, in_group = first * SLAB_K - start * p.group;
             for (int i = 0; i < slabs_here; i++) {
                 ok &= mbar_wait<LONG_WAIT>(smem_u32(&raw_empty[s]), ph ^ 1, &gave_up);
@@ -445,7 +479,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                     mbar_expect_tx(fb, PACKED_BYTES);
                     tma_load_2d(at, &map_w, fb, (first + i) * SLAB_K / 2, n0);
                 }
-                Scales::copy(at + PACKED_BYTES, scales, zeros, n0, p.N, p.groups, start, lane);
+                copies(at + PACKED_BYTES, start, lane, p.aligned);
                 copies_arrive(fb);
                 for (in_group += SLAB_K; in_group >= p.group; in_group -= p.group) start++;
                 if (++s == p.raws) s = 0, ph ^= 1;
@@ -520,9 +554,9 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                         for (int k = in_start + team * TILE_K + h * UNIT_K; k >= p.group; k -= p.group) ahead++;
                     }
                     const bool in = start + ahead < groups;   // past the end of K: X is zero there, and so is the scale
-                    const uint32_t scale = Scales::scale_bits(stage + PACKED_BYTES, row, row_group, start, ahead);
+                    const uint32_t scale = Scales::scale_bits(stage + PACKED_BYTES, row, row_group, start, ahead, p.aligned);
                     s2[h] = in ? scale * 0x10001u : 0u;
-                    z2[h] = MAGIC<T> + 0x10001u * (ZEROS && in ? Scales::zero(stage + PACKED_BYTES, row, row_group, start, ahead) : 8);
+                    z2[h] = MAGIC<T> + 0x10001u * (ZEROS && in ? Scales::zero(stage + PACKED_BYTES, row, row_group, start, ahead, p.aligned) : 8);
                 }
                 if (PARTS == 1) s2[1] = s2[0], z2[1] = z2[0];
                 if (whole) start += SLAB_K / 32 >> whole_shift;
@@ -633,7 +667,7 @@ constexpr CUtensorMapDataType MAP_TYPE = std::is_same_v<T, __half> ? CU_TENSOR_M
 
 template <class T, int NT, int FLUSH, bool ZEROS>
 int launch_few(const Args& p) {
-    constexpr int TOKENS = 8 * NT, smem = few::smem_of<NT>();
+    constexpr int TOKENS = 8 * NT, smem = few::Stage<T, NT, FLUSH, ZEROS>::SMEM;
     constexpr auto kern = few::matmul_w4_kernel<T, NT, FLUSH, ZEROS>;
     if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
     const int tiles_n = (p.N - 1) / ROWS + 1, slabs = (p.K - 1) / few::SLAB_K + 1, groups = (p.K - 1) / p.group + 1;
@@ -649,7 +683,7 @@ int launch_few(const Args& p) {
             return rc;
         const dim3 grid(tiles_n << shift, (rows - 1) / TOKENS + 1);
         if (const int rc = basalt_k::launch_clusters(WHO, kern, grid, few::THREADS, smem, 1 << shift, p.stream, mw, mx, (const T*)p.scales, p.zeros, (T*)p.c + m * p.ldc, p.ldc, rows,
-                                                     p.N, p.K, p.group, groups, shift, p.status))
+                                                     p.N, p.K, p.group, groups, (int)SlabScales<T, FLUSH, ZEROS>::aligned(p.scales, p.zeros, p.group, groups), shift, p.status))
             return rc;
     }
     return 0;
@@ -659,7 +693,8 @@ template <class T, int FLUSH, bool ZEROS>
 int launch_tall(const Args& p) {
     constexpr int RAW_BYTES = tall::PACKED_BYTES + SlabScales<T, FLUSH, ZEROS>::BYTES;
     const int sms = basalt_k::sm_count(), slabs = (p.K - 1) / tall::SLAB_K + 1;
-    tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0, (p.K - 1) / p.group + 1, 0};
+    tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0, (p.K - 1) / p.group + 1, 0, 0};
+    q.aligned = SlabScales<T, FLUSH, ZEROS>::aligned(p.scales, p.zeros, p.group, q.groups);
     // The width of a tile: of the few counts of tiles over M that come near 256 columns each the one whose rounds over the SMs
     // cost least. A slab costs two clocks a column, and not less than the unpacking of its weights, about 112 columns' worth.
     int64_t best = INT64_MAX;

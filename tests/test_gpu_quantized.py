@@ -259,7 +259,7 @@ def w4_weights(g, N, K, group, zeros, t, exact):
 
 
 W4_SHAPES = [(1, 1, 1, 32), (1, 128, 256, 128), (2, 127, 33, 32), (8, 130, 255, 64), (9, 64, 257, 128), (16, 300, 1000, 32), (17, 129, 512, 96), (32, 200, 2048, 128), (33, 140, 300, 64),
-             (70, 260, 640, 128), (129, 128, 384, 1024), (200, 300, 1111, 128), (1, 500, 8192, 128), (3, 96, 4096, 64), (1, 140, 16000, 32), (2, 20000, 4500, 128), (13, 19000, 4100, 64), (20, 260, 17000, 96), (31, 20000, 2200, 32), (9, 7000, 129, 128)]
+             (70, 260, 640, 128), (129, 128, 384, 1024), (200, 300, 1111, 128), (1, 500, 8192, 128), (3, 96, 4096, 64), (1, 140, 16000, 32), (2, 20000, 4500, 128), (13, 19000, 4100, 64), (20, 260, 17000, 96), (31, 20000, 2200, 32), (9, 7000, 129, 128), (5, 129, 2560, 256), (40, 300, 2816, 256), (6, 131, 2048, 64), (70, 130, 4096, 32), (3, 128, 1024, 192)]
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])
