@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_bar;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t gave_up;
+    __shared__ float scale[TN];   // of the tile's rows of A: in the epilogue each would be a trip to memory
     const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int splits = 1 << shift, split = blockIdx.x & (splits - 1), n0 = (blockIdx.x >> shift) * BN, m0 = blockIdx.y * TN;
@@ -73,6 +74,8 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         mbar_init(smem_u32(&acc_bar), 1);
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -87,6 +90,9 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     wait_for_predecessor();
     if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
+    for (int m = threadIdx.x; m < TN; m += THREADS) scale[m] = m0 + m < M ? a_scales[m0 + m] : 0.0f;
+    const float b_scale = n0 + (int)threadIdx.x < N ? b_scales[n0 + threadIdx.x] : 0.0f;
+    __syncthreads();
 
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < count; i++) {
@@ -122,39 +128,40 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
 
     ok &= mbar_wait(smem_u32(&acc_bar), 0, &gave_up);   // on give-up the drain still runs (warp-uniformly) on whatever TMEM holds
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const int n = n0 + threadIdx.x, tokens = min(TN, M - m0);
+    const int n = n0 + threadIdx.x, tokens = min(TN, M - m0), each = TN >> shift;
     const uint32_t src = tmem_acc + ((uint32_t)(warp * 32) << 16);
-    const float b_scale = n < N ? b_scales[n] : 0.0f;
-    float* sums = reinterpret_cast<float*>(smem_raw + (tiles - smem_u32(smem_raw)));
-    if (splits > 1) __syncthreads();   // every wait on the ring is over: its memory takes the partial sums
+    if (splits > 1) {   // every CTA of the cluster is through with its ring, whose memory takes the partial sums
+        __syncwarp();
+        cluster_sync_all();
+    }
+    const uint32_t mine = tiles + (split * each * BN + threadIdx.x) * 4;   // in the CTA that adds up column c: [CTA][c >> shift][row of B]
 #pragma unroll 1
     for (int c = 0; c < TN; c += 16) {
         if (c >= tokens) break;
         uint32_t r[16];
         __syncwarp();   // the load is the whole warp's
         tmem_load_16(src + (uint32_t)c, r);
-        if (splits > 1) {
+        if (splits > 1) {   // stores that nobody waits for, and not loads: the way between two SMs' memories is paid once, at the barrier
 #pragma unroll
-            for (int j = 0; j < 16; j++) sums[(c + j) * BN + threadIdx.x] = __uint_as_float(r[j]);
+            for (int j = 0; j < 16; j++)
+                if (c + j < tokens) store_cluster_f32(map_to_cta(mine + ((c + j) >> shift) * BN * 4, (c + j) & (splits - 1)), __uint_as_float(r[j]));
         } else if (n < N) {
 #pragma unroll
             for (int j = 0; j < 16; j++)
-                if (c + j < tokens) store_as(C + (m0 + c + j) * ldc + n, __uint_as_float(r[j]) * a_scales[m0 + c + j] * b_scale);
+                if (c + j < tokens) store_as(C + (m0 + c + j) * ldc + n, __uint_as_float(r[j]) * scale[c + j] * b_scale);
         }
     }
     if (splits > 1) {
         __syncwarp();
         cluster_sync_all();
+        const float* sums = reinterpret_cast<const float*>(smem_raw + (tiles - smem_u32(smem_raw)));
         if (n < N) {
             for (int c = split; c < tokens; c += splits) {
-                const uint32_t at = smem_u32(&sums[c * BN + threadIdx.x]);
                 float total = 0.0f;
-                for (int q = 0; q < splits; q++) total += load_cluster_f32(map_to_cta(at, q));
-                store_as(C + (m0 + c) * ldc + n, total * a_scales[m0 + c] * b_scale);
+                for (int q = 0; q < splits; q++) total += sums[(q * each + (c >> shift)) * BN + threadIdx.x];
+                store_as(C + (m0 + c) * ldc + n, total * scale[c] * b_scale);
             }
         }
-        __syncwarp();
-        cluster_sync_all();   // no CTA leaves while another reads its sums
     }
     if (!ok && status) atomicExch(status, 1);
 
@@ -354,6 +361,13 @@ struct Args {
 
 const char* const WHO = "matmul_e4m3";
 
+// How many CTAs share a tile's K, as a power of two: two CTAs fit an SM; split while the tiles leave room and every share keeps four slabs.
+int split_shift(int64_t tiles, int slabs) {
+    int shift = 0;
+    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && slabs >= 8 << shift) shift++;
+    return shift;
+}
+
 template <class T, int TN>
 int launch(const Args& p) {
     CUtensorMap ma, mb;
@@ -364,9 +378,8 @@ int launch(const Args& p) {
     if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
     const int tiles_n = (p.N - 1) / BN + 1, slabs = (p.K - 1) / BK + 1;
     const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TN + 1);
-    int shift = 0;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps four slabs
-    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && slabs >= 8 << shift) shift++;
-    const dim3 grid(tiles_n << shift, (p.M - 1) / TN + 1);   // M is at most 256 here
+    const int shift = split_shift(tiles, slabs);
+    const dim3 grid(tiles_n << shift, (p.M - 1) / TN + 1);
     return basalt_k::launch_clusters(WHO, kern, grid, THREADS, smem, 1 << shift, p.stream, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, shift, p.status);
 }
 
@@ -383,16 +396,41 @@ int launch_pair(const Args& p) {
     return basalt_k::launch_clusters(WHO, kern, 2 * pairs, pair::PAIR_THREADS, pair::SMEM, 2, p.stream, ma, mb, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, p.status);
 }
 
+// What a call takes, in microseconds, by the kernel above with tiles of TN rows of A: a slab takes a round of CTAs 0.31 to 0.51; the weights
+// come from memory at 6.3 TB/s, and a third of them again for each further tile over M; the join of a split tile takes 0.055 a column.
+// (Measured / estimated: 8192 x 8192 for 1 row 15.0 / 13.9, 64 rows 19.5 / 18.2; 4096 x 4096 for 64 rows in tiles of 16, 32
+// and 64: 10.5 / 10.3, 8.8 / 9.4, 9.3 / 10.2; for 128 rows 13.5 / 13.1, 12.6 / 11.2, 11.4 / 11.1 and in tiles of 128 12.9 / 13.7.)
+double time_of_tiles(int M, int N, int K, int TN) {
+    const int64_t tiles_m = (M - 1) / TN + 1, tiles = tiles_m * ((N - 1) / BN + 1), slabs = (K - 1) / BK + 1;
+    const int shift = split_shift(tiles, (int)slabs);
+    const double slab = TN == 16 ? 0.31 : TN == 32 ? 0.32 : TN == 64 ? 0.37 : 0.51;
+    const double rounds = (double)(((tiles << shift) - 1) / (2 * basalt_k::sm_count()) + 1), compute = rounds * slab * (double)((slabs - 1 >> shift) + 1);
+    const double memory = (double)N * K * (1.0 + 0.35 * (double)(tiles_m - 1)) / 6.3e6;
+    return 3.2 + (compute > memory ? compute : memory) + (shift ? 1.5 + 0.055 * (M < TN ? M : TN) : 0.0);
+}
+// By the pairs of CTAs: 0.305 a slab and round of 74 tiles. (4096 x 4096 for 256 rows 15.0 / 15.3, where tiles of 32 rows take 14.0; 8192 x 8192
+// for 256 rows 25.5 / 25.0, where tiles of 64 take 27.3; for 2048 rows 84 / 83.6, where tiles of 128 take 142.)
+double time_of_pairs(int M, int N, int K) {
+    const int64_t tiles = (int64_t)((M - 1) / pair::TM + 1) * ((N - 1) / pair::TN + 1);
+    return 5.5 + 0.305 * (double)((tiles - 1) / (basalt_k::sm_count() / 2) + 1) * (double)((K - 1) / BK + 1);
+}
+
 template <class T>
 int launch_type(const Args& p) {
-    if (p.M > 256) {
-        const bool vectors = (uintptr_t)p.c % 16 == 0 && p.ldc * sizeof(T) % 16 == 0;
-        return vectors ? launch_pair<T, true>(p) : launch_pair<T, false>(p);
+    int best = 0;
+    double least = time_of_pairs(p.M, p.N, p.K);
+    for (int TN = 16; TN <= 128; TN *= 2) {
+        if (TN > 16 && TN >= 2 * p.M) break;
+        if ((p.M - 1) / TN >= 65535) continue;   // a grid's second dimension
+        const double t = time_of_tiles(p.M, p.N, p.K, TN);
+        if (t < least) least = t, best = TN;
     }
-    if (p.M <= 16) return launch<T, 16>(p);
-    if (p.M <= 32) return launch<T, 32>(p);
-    if (p.M <= 64) return launch<T, 64>(p);
-    return launch<T, 128>(p);
+    if (best == 16) return launch<T, 16>(p);
+    if (best == 32) return launch<T, 32>(p);
+    if (best == 64) return launch<T, 64>(p);
+    if (best == 128) return launch<T, 128>(p);
+    const bool vectors = (uintptr_t)p.c % 16 == 0 && p.ldc * sizeof(T) % 16 == 0;
+    return vectors ? launch_pair<T, true>(p) : launch_pair<T, false>(p);
 }
 
 }  // namespace
