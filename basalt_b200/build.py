@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libbasalt_b200.so")
 CLI = os.path.join(HERE, "basalt-b200")
+PYTHON_BINDING = os.path.join(HERE, "_klaunch.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 CXX_SOURCES = ["bir.cpp", "passes.cpp", "emit.cpp", "emit_mma.cpp", "regbudget.cpp", "frontend_c.cpp", "frontend_triton.cpp", "capi.cpp", "runtime.cpp"]
@@ -68,6 +70,14 @@ def _build_shims(force: bool, run) -> None:
                  "-Wl,-rpath,$ORIGIN", "-lpthread"])
 
 
+def _build_python_binding(force: bool, run) -> None:
+    """_klaunch.so: the CPython binding of the launch-bound kernels, linked against the library beside it."""
+    src = os.path.join(CSRC, "python_binding.cpp")
+    if force or _stale(PYTHON_BINDING, [src, LIB, os.path.abspath(__file__)]):
+        run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{sysconfig.get_paths()['include']}", "-o", PYTHON_BINDING, src, f"-L{HERE}",
+             "-lbasalt_b200", "-Wl,-rpath,$ORIGIN"])
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.abspath(__file__)]
@@ -96,6 +106,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or jobs or _stale(LIB, objs):
         run([nvcc, "-shared", "-o", LIB, *objs, "-cudart", "static", "-Xlinker", "--no-undefined", "-ldl", "-lpthread", "-lrt"])
     _build_shims(force, run)
+    _build_python_binding(force, run)
     cli_src = os.path.join(CSRC, "cli.cpp")
     if force or _stale(CLI, [cli_src, LIB]):
         run(["g++", "-std=c++17", "-O2", "-o", CLI, cli_src, f"-L{HERE}", "-lbasalt_b200", "-Wl,-rpath,$ORIGIN"])

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 
+from . import _klaunch
 from ._lib import lib
 from .runtime import DeviceBuffer
 
@@ -93,40 +94,33 @@ def sgemm_f32_variant(A, B, Cm, M: int, N: int, K: int, no_tail_split: bool = Fa
 TYPES = {"f16": 0, "bf16": 1, "f32": 2}
 
 
-def _address(x):
-    """A device pointer, a DeviceBuffer or None, as ctypes takes it for a pointer argument."""
-    return x.device_ptr() if isinstance(x, DeviceBuffer) else x
-
-
 def _type(name: str) -> int:
     if name not in TYPES:
         raise KernelError(f"unknown type {name!r}: one of {', '.join(TYPES)}")
     return TYPES[name]
 
 
+# The four below go through a CPython binding instead of ctypes, whose conversion of their arguments would take longer than the launch.
+# Pointers are ints, DeviceBuffers or None.
+
 def rms_norm(x, y, rows: int, cols: int, dtype: str, weight=None, eps: float = 1e-6, residual=None, total=None, scales=None, ldx=None, ldy=None,
              ldr=None, ldt=None, stream=None):
     """y = (x + residual) * weight / rms over rows of `dtype`; `total` receives x + residual. With `scales` (f32, one a row) y is
     e4m3, y / scales[row]. Strides are in elements and default to cols."""
-    _check(lib.basalt_k_rms_norm(_type(dtype), _address(x), cols if ldx is None else ldx, _address(residual), cols if ldr is None else ldr, _address(total),
-                                 cols if ldt is None else ldt, _address(weight), eps, _address(y), cols if ldy is None else ldy, _address(scales), rows, cols,
-                                 stream))
+    _check(_klaunch.rms_norm(_type(dtype), x, ldx, residual, ldr, total, ldt, weight, eps, y, ldy, scales, rows, cols, stream))
 
 
 def quantize_e4m3(x, q, scales, rows: int, cols: int, dtype: str, ldx=None, ldq=None, stream=None):
     """q = e4m3(x / scales[row]) with scales[row] = max|x| / 448, row by row."""
-    _check(lib.basalt_k_quantize_e4m3(_type(dtype), _address(x), cols if ldx is None else ldx, _address(q), cols if ldq is None else ldq, _address(scales), rows,
-                                      cols, stream))
+    _check(_klaunch.quantize_e4m3(_type(dtype), x, ldx, q, ldq, scales, rows, cols, stream))
 
 
 def matmul_e4m3(A, a_scales, B, b_scales, Cm, M: int, N: int, K: int, out: str = "f16", lda=None, ldb=None, ldc=None, status=None, stream=None):
     """C = (A * B^T) * a_scales[m] * b_scales[n] of e4m3 A [M x K] and B [N x K]; C of type `out`. Row strides default to K, K and N."""
-    _check(lib.basalt_k_matmul_e4m3(_address(A), K if lda is None else lda, _address(a_scales), _address(B), K if ldb is None else ldb, _address(b_scales), _type(out),
-                                    _address(Cm), N if ldc is None else ldc, M, N, K, _address(status), stream))
+    _check(_klaunch.matmul_e4m3(A, lda, a_scales, B, ldb, b_scales, _type(out), Cm, ldc, M, N, K, status, stream))
 
 
 def matmul_w4(X, W, scales, Cm, M: int, N: int, K: int, group: int, dtype: str = "f16", zeros=None, ldx=None, ldw=None, ldc=None, status=None, stream=None):
     """C = X * ((q - zeros) * scales)^T with 4-bit q packed two to a byte in W [N x K/2], scales and zeros per `group` of k.
     ldx and ldc count elements, ldw bytes; they default to K, N and the packed row."""
-    _check(lib.basalt_k_matmul_w4(_type(dtype), _address(X), K if ldx is None else ldx, _address(W), (K + 1) // 2 if ldw is None else ldw, _address(scales),
-                                  _address(zeros), group, _address(Cm), N if ldc is None else ldc, M, N, K, _address(status), stream))
+    _check(_klaunch.matmul_w4(_type(dtype), X, ldx, W, ldw, scales, zeros, group, Cm, ldc, M, N, K, status, stream))

@@ -179,7 +179,8 @@ def run_e4m3(gpu, a, sa, b, sb, K, out, ldc_pad=3):
 
 
 E4M3_SHAPES = [(1, 1, 1), (1, 128, 128), (2, 127, 16), (7, 129, 31), (16, 300, 127), (17, 64, 129), (33, 260, 1000), (64, 128, 2048), (65, 257, 640), (129, 130, 256), (200, 520, 515),
-               (256, 256, 128), (300, 700, 1152), (515, 512, 384), (1, 1000, 8192), (5, 200, 16384)]
+               (256, 256, 128), (300, 700, 1152), (515, 512, 384), (1, 1000, 8192), (5, 200, 16384), (20, 9000, 2100), (250, 3000, 2200), (120, 4100, 4200), (1000, 2000, 1500),
+               (600, 4000, 300), (65, 4100, 4200), (2600, 2100, 1000)]   # the last ones: each tile width with K whole and shared, and pairs of CTAs
 
 
 @pytest.mark.parametrize("out", ["f32", "f16"])
@@ -197,7 +198,7 @@ def test_matmul_e4m3_exact_on_small_integers(gpu, shape, out):
 
 
 @pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("shape", [(1, 300, 4096), (19, 129, 777), (130, 400, 2049), (384, 640, 1024)])
+@pytest.mark.parametrize("shape", [(1, 300, 4096), (19, 129, 777), (130, 400, 2049), (384, 640, 1024), (2600, 2104, 999)])
 def test_matmul_e4m3_random(gpu, shape, out):
     M, N, K = shape
     g = gen(K)

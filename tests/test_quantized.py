@@ -1,5 +1,6 @@
 """What the norm, the row quantisation and the e4m3 and 4-bit products refuse. Every check here comes before
 anything that needs a device, so the refusals run on a machine without one."""
+import numpy as np
 import pytest
 
 from basalt_b200 import kernels
@@ -116,3 +117,17 @@ def test_nothing_to_do_is_no_error():
     kernels.matmul_e4m3(X, S, Y, S, Z, 0, 8, 64)
     kernels.matmul_e4m3(X, S, Y, S, Z, 4, 0, 64)
     kernels.matmul_w4(X, Y, S, Z, 0, 8, 64, 32)
+
+
+def test_arguments_that_fit_no_parameter():
+    with pytest.raises(OverflowError):
+        kernels.matmul_w4(X, Y, S, Z, 2**32 + 1, 8, 64, 32)     # must not wrap to one row
+    with pytest.raises(OverflowError):
+        kernels.rms_norm(-16, Y, 1, 64, "f16")
+    with pytest.raises(TypeError):
+        kernels.quantize_e4m3(X, Y, S, None, 64, "f16")
+    with pytest.raises(TypeError):
+        norm(eps="small")
+    with pytest.raises(AttributeError):
+        norm(x="x")
+    norm(x=np.uint64(X), rows=np.int64(0))                       # whatever is an integer passes
