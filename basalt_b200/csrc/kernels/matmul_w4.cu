@@ -19,6 +19,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+#include <string.h>
 
 #include <type_traits>
 
@@ -270,26 +271,40 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
         // lanes exchange them.
         const int my_row = row0 + g + 8 * t;
         const uint32_t row_group = (uint32_t)min(n0 + my_row, N - 1) * (uint32_t)groups;
-        int start = first_group, in_start = first * SLAB_K - start * group;
+        int start = first_group, in_start = first * SLAB_K - start * group, s = 0;
+        uint32_t ph = 0;
         for (int i = 0; i < count; i++) {
-            const int s = i % STAGES;
-            ok &= mbar_wait(smem_u32(&full_bar[s]), (i / STAGES) & 1, &gave_up);
+            ok &= mbar_wait(smem_u32(&full_bar[s]), ph, &gave_up);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const uint8_t* my_scales = smem + s * STAGE_BYTES + S::SCALES;
             float by[4 / FLUSH];
             Zero<T> z[ZEROS ? 4 / FLUSH : 1];
             if (!ZEROS) z[0].set(8);
-            int ahead = 0, k = in_start + half * 128;   // the group of this half's next part, counted from the slab's first
+            if (aligned) {   // this half's groups follow one another, and all of them exist
+                const uint8_t* from = my_scales + my_row * 2 * Scales::GROUPS + half * Scales::GROUPS;
+                T scale[4 / FLUSH];
+                memcpy(scale, __builtin_assume_aligned(from, sizeof scale), sizeof scale);
 #pragma unroll
-            for (int f = 0; f < 4 / FLUSH; f++) {
-                for (; k >= group; k -= group) ahead++;
-                const bool in = start + ahead < groups;   // past the end of K: X is zero there, and so is the scale
-                by[f] = in ? to_float(as_type<T>(Scales::scale_bits(my_scales, my_row, row_group, start, ahead, aligned))) : 0.0f;
-                if (ZEROS) z[f].set(in ? Scales::zero(my_scales, my_row, row_group, start, ahead, aligned) : 0);
-                k += FLUSH * UNIT_K;
+                for (int f = 0; f < 4 / FLUSH; f++) by[f] = to_float(scale[f]);
+                if constexpr (ZEROS) {
+                    const uint8_t* zero = my_scales + Scales::ZERO_AT + my_row * Scales::ZERO_PIECE + ((row_group + start) & (Scales::ZERO_PIECE - 1)) + half * (Scales::GROUPS / 2);
+#pragma unroll
+                    for (int f = 0; f < 4 / FLUSH; f++) z[f].set(zero[f]);
+                }
+                start += Scales::GROUPS;
+            } else {
+                int ahead = 0, k = in_start + half * 128;   // the group of this half's next part, counted from the slab's first
+#pragma unroll
+                for (int f = 0; f < 4 / FLUSH; f++) {
+                    for (; k >= group; k -= group) ahead++;
+                    const bool in = start + ahead < groups;   // past the end of K: X is zero there, and so is the scale
+                    by[f] = in ? to_float(as_type<T>(Scales::scale_bits(my_scales, my_row, row_group, start, ahead, false))) : 0.0f;
+                    if (ZEROS) z[f].set(in ? Scales::zero(my_scales, my_row, row_group, start, ahead, false) : 0);
+                    k += FLUSH * UNIT_K;
+                }
+                for (in_start += SLAB_K; in_start >= group; in_start -= group) start++;
             }
-            for (in_start += SLAB_K; in_start >= group; in_start -= group) start++;
             const uint8_t* w_at = smem + s * STAGE_BYTES + (row0 + g) * 128 + t * 4;
             const uint8_t* x_at = smem + s * STAGE_BYTES + S::X + half * 4 * TOKENS * X_BOX_K * 2 + lane * 16;
 #pragma unroll
@@ -327,6 +342,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
+            if (++s == STAGES) s = 0, ph ^= 1;
         }
     }
 
