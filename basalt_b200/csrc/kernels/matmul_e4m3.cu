@@ -44,12 +44,14 @@ __device__ __forceinline__ uint32_t two_as(float a, float b) {
 }
 
 template <int TN>
-__host__ __device__ constexpr int stages_of() { return TN <= 32 ? 5 : TN == 64 ? 4 : 3; }   // at most 96 KB: two CTAs fit an SM
+__host__ __device__ constexpr int stages_of() { return TN == 16 ? 5 : TN <= 64 ? 4 : 3; }
 template <int TN>
-__host__ __device__ constexpr int smem_of() {
-    constexpr int ring = stages_of<TN>() * (B_BYTES + TN * BK), sums = TN * BN * 4;
-    return (ring > sums ? ring : sums) + 1024;
-}
+__host__ __device__ constexpr int ring_of() { return stages_of<TN>() * (B_BYTES + TN * BK); }
+// Where the partial sums of a cluster meet: behind the ring where there is room, so that no CTA waits for the others' rings; else in it.
+template <int TN>
+__host__ __device__ constexpr int sums_at() { return TN <= 32 ? ring_of<TN>() : 0; }
+template <int TN>
+__host__ __device__ constexpr int smem_of() { return ring_of<TN>() + (TN <= 32 ? TN * BN * 4 : 0) + 1024; }   // at most 99 KB: two CTAs fit an SM
 
 template <class T, int TN>
 __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
@@ -85,6 +87,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    cluster_arrive();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_acc = tmem_slot;
     wait_for_predecessor();
@@ -130,11 +133,10 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const int n = n0 + threadIdx.x, tokens = min(TN, M - m0), each = TN >> shift;
     const uint32_t src = tmem_acc + ((uint32_t)(warp * 32) << 16);
-    if (splits > 1) {   // every CTA of the cluster is through with its ring, whose memory takes the partial sums
-        __syncwarp();
-        cluster_sync_all();
-    }
-    const uint32_t mine = tiles + (split * each * BN + threadIdx.x) * 4;   // in the CTA that adds up column c: [CTA][c >> shift][row of B]
+    __syncwarp();
+    cluster_wait();   // every CTA of the cluster runs, so its shared memory is there
+    if (splits > 1 && sums_at<TN>() == 0) cluster_sync_all();   // and is through with its ring
+    const uint32_t mine = tiles + sums_at<TN>() + (split * each * BN + threadIdx.x) * 4;   // in the CTA that adds up column c: [CTA][c >> shift][row of B]
 #pragma unroll 1
     for (int c = 0; c < TN; c += 16) {
         if (c >= tokens) break;
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     if (splits > 1) {
         __syncwarp();
         cluster_sync_all();
-        const float* sums = reinterpret_cast<const float*>(smem_raw + (tiles - smem_u32(smem_raw)));
+        const float* sums = reinterpret_cast<const float*>(smem_raw + (tiles - smem_u32(smem_raw)) + sums_at<TN>());
         if (n < N) {
             for (int c = split; c < tokens; c += splits) {
                 float total = 0.0f;
@@ -408,11 +410,12 @@ double time_of_tiles(int M, int N, int K, int TN) {
     const double memory = (double)N * K * (1.0 + 0.35 * (double)(tiles_m - 1)) / 6.3e6;
     return 3.2 + (compute > memory ? compute : memory) + (shift ? 1.5 + 0.055 * (M < TN ? M : TN) : 0.0);
 }
-// By the pairs of CTAs: 0.305 a slab and round of 74 tiles. (4096 x 4096 for 256 rows 15.0 / 15.3, where tiles of 32 rows take 14.0; 8192 x 8192
+// By the pairs of CTAs: 0.305 a slab and round of 74 tiles, and the weights at 5.4 TB/s. (16384 x 16384 for 64 rows 52.7 / 55.2; 4096 x 4096 for 256 rows 15.0 / 15.3, where tiles of 32 rows take 14.0; 8192 x 8192
 // for 256 rows 25.5 / 25.0, where tiles of 64 take 27.3; for 2048 rows 84 / 83.6, where tiles of 128 take 142.)
 double time_of_pairs(int M, int N, int K) {
     const int64_t tiles = (int64_t)((M - 1) / pair::TM + 1) * ((N - 1) / pair::TN + 1);
-    return 5.5 + 0.305 * (double)((tiles - 1) / (basalt_k::sm_count() / 2) + 1) * (double)((K - 1) / BK + 1);
+    const double compute = 0.305 * (double)((tiles - 1) / (basalt_k::sm_count() / 2) + 1) * (double)((K - 1) / BK + 1), memory = (double)N * K / 5.4e6;
+    return 5.5 + (compute > memory ? compute : memory);
 }
 
 template <class T>
