@@ -392,7 +392,7 @@ constexpr int SLAB_K = 256, TILE_K = 64, PACKED_BYTES = ROWS * SLAB_K / 2, MAX_S
 constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, TEAMS = SLAB_K / TILE_K, TEAM = 4, FIRST_UNPACKER = 4, EPILOGUE = 4;
 constexpr int FIRST_EPILOGUE = FIRST_UNPACKER + TEAMS * TEAM;
 constexpr int TALL_THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE), SMEM_MOST = 231936;
-// Tensor memory: 256 columns of accumulators (two of up to 128, or one), and 32 columns a stage for 64 k of unpacked weights.
+// Tensor memory: 256 columns of accumulators (two of up to 128, or one), and 32 columns for each 64 k of unpacked weights in a stage.
 constexpr uint32_t TMEM_COLS = 512, WEIGHTS_AT = 256, WEIGHT_COLS = TILE_K / 2;
 
 // Eight packed weights of one group -> (q - z) * s in the order of k, two to a register.
@@ -411,12 +411,14 @@ struct Shape {
     int M, N, K, group, tile_m, tiles_n, tiles, stages, raws, groups, split_shift, aligned;
 };
 
-template <class T, int FLUSH, bool ZEROS>
+// HALVES: 64-k tiles in a stage. Two, where the tile is narrow: the thread that issues the MMAs needs some 250 clocks a stage beside them,
+// more than the products of 64 k take there (64 rows, 8192 x 8192: 24.5 us with one, HALVES_HERE with two).
+template <class T, int FLUSH, bool ZEROS, int HALVES>
 __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                   const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C,
                                                                   int64_t ldc, const Shape p, int32_t* status) {
     using Scales = SlabScales<T, FLUSH, ZEROS>;
-    constexpr int RAW_BYTES = PACKED_BYTES + Scales::BYTES;
+    constexpr int RAW_BYTES = PACKED_BYTES + Scales::BYTES, STAGE_K = TILE_K * HALVES, STAGE_COLS = WEIGHT_COLS * HALVES, SLAB_STAGES = SLAB_K / STAGE_K;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], raw_full[MAX_RAW], raw_empty[MAX_RAW], tfull_bar[2], tempty_bar[2];
     __shared__ uint32_t tmem_slot;
@@ -427,14 +429,14 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     const int shift = p.split_shift, splits = 1 << shift, split = blockIdx.x & (splits - 1);
     const int my_tile = blockIdx.x >> shift, step = gridDim.x >> shift;
     const int slabs = (p.K - 1) / SLAB_K + 1, first = slabs * split >> shift, slabs_here = (slabs * (split + 1) >> shift) - first;
-    const int count = min(slabs_here * (SLAB_K / TILE_K), (p.K - 1) / TILE_K + 1 - first * (SLAB_K / TILE_K));   // tiles of 64 k
+    const int count = min(slabs_here * SLAB_STAGES, (p.K - 1) / STAGE_K + 1 - first * SLAB_STAGES);
     const int first_group = (unsigned)(first * SLAB_K) / (unsigned)p.group;
-    const int stage_bytes = p.tile_m * TILE_K * 2, accs = p.tile_m <= 128 ? 2 : 1;   // with one accumulator, its drain is not hidden
+    const int half_bytes = p.tile_m * TILE_K * 2, stage_bytes = half_bytes * HALVES, accs = p.tile_m <= 128 ? 2 : 1;   // with one accumulator, its drain is not hidden
 
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int s = 0; s < p.stages; s++) {
-            mbar_init(smem_u32(&full_bar[s]), 1 + TEAM);   // the rows of X, and each warp of the team that unpacks it
+            mbar_init(smem_u32(&full_bar[s]), 1 + TEAM * HALVES);   // the rows of X, and each warp of the teams that unpack it
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int s = 0; s < p.raws; s++) {
@@ -471,7 +473,8 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                     if (!ok) break;
                     const uint32_t fb = smem_u32(&full_bar[s]);
                     mbar_expect_tx(fb, stage_bytes);
-                    tma_load_2d(ring + s * stage_bytes, &map_x, fb, first * SLAB_K + i * TILE_K, m0);
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) tma_load_2d(ring + s * stage_bytes + h * half_bytes, &map_x, fb, first * SLAB_K + i * STAGE_K + h * TILE_K, m0);
                     if (++s == p.stages) s = 0, ph ^= 1;
                 }
             }
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
         const uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
         const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(p.tile_m >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
         const uint32_t full0 = smem_u32(&full_bar[0]), empty0 = smem_u32(&empty_bar[0]), end = full0 + 8 * p.stages, w0 = tmem_base + WEIGHTS_AT;
-        const uint64_t x0 = smem_desc(ring, 16, 1024), x_step = stage_bytes >> 4;
+        const uint64_t x0 = smem_desc(ring, 16, 1024), x_step = stage_bytes >> 4, x_half = half_bytes >> 4;
         uint32_t bar = full0, w = w0, ph = 0, buf = 0, use = 0;
         uint64_t x = x0;
         for (int t = my_tile; t < p.tiles; t += step) {
@@ -524,12 +527,16 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                 ok &= mbar_wait(bar, ph, &gave_up);
                 __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                umma_f16_tmem(acc, w, x, idesc, accumulate);
-                accumulate = 1;
 #pragma unroll
-                for (int k = 1; k < TILE_K / 16; k++) umma_f16_tmem(acc, w + 8 * k, x + (uint64_t)(2 * k), idesc, 1);
+                for (int h = 0; h < HALVES; h++) {
+#pragma unroll
+                    for (int k = 0; k < TILE_K / 16; k++) {
+                        umma_f16_tmem(acc, w + h * WEIGHT_COLS + 8 * k, x + h * x_half + (uint64_t)(2 * k), idesc, accumulate);
+                        accumulate = 1;
+                    }
+                }
                 umma_commit_elected(bar - full0 + empty0);
-                bar += 8, w += WEIGHT_COLS, x += x_step;
+                bar += 8, w += STAGE_COLS, x += x_step;
                 if (bar == end) bar = full0, w = w0, x = x0, ph ^= 1;
             }
             umma_commit_elected(smem_u32(&tfull_bar[buf]));
@@ -555,7 +562,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             const uint32_t row_group = (uint32_t)min(t % p.tiles_n * ROWS + row, p.N - 1) * (uint32_t)groups;
             int place = at, start = first_group, in_start = first * SLAB_K - start * p.group;
             uint32_t parity = ph;
-            forward(place, parity, team);
+            forward(place, parity, team / HALVES);
             for (int j = 0; j < slabs_here; j++) {
                 ok &= mbar_wait(smem_u32(&raw_full[rs]), rph, &gave_up);
                 ok = __all_sync(0xffffffffu, ok);
@@ -587,16 +594,16 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&raw_empty[rs]));
                 if (++rs == p.raws) rs = 0, rph ^= 1;
-                if (4 * j + team >= count) continue;   // this tile lies behind the end of K
+                if (j * SLAB_STAGES + team / HALVES >= count) continue;   // this stage lies behind the end of K
                 ok &= mbar_wait(smem_u32(&empty_bar[place]), parity ^ 1, &gave_up);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                tmem_store_32(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + WEIGHTS_AT + place * WEIGHT_COLS, out);
+                tmem_store_32(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + WEIGHTS_AT + place * STAGE_COLS + team % HALVES * WEIGHT_COLS, out);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&full_bar[place]));
-                forward(place, parity, TEAMS);
+                forward(place, parity, SLAB_STAGES);
             }
             forward(at, ph, count);
         }
@@ -711,29 +718,35 @@ int launch_tall(const Args& p) {
     const int sms = basalt_k::sm_count(), slabs = (p.K - 1) / tall::SLAB_K + 1;
     tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0, (p.K - 1) / p.group + 1, 0, 0};
     q.aligned = SlabScales<T, FLUSH, ZEROS>::aligned(p.scales, p.zeros, p.group, q.groups);
-    // The width of a tile: of the few counts of tiles over M that come near 256 columns each the one whose rounds over the SMs
-    // cost least. A slab costs two clocks a column, and not less than the unpacking of its weights, about 112 columns' worth.
+    // The width of a tile and the CTAs that share its K (one CTA fits an SM): of the few counts of tiles over M that come near
+    // 256 columns each, the one that costs least. A slab costs what its products do, two clocks a column and 64 k, and not less than
+    // its unpacking, about 112 columns' worth; a join costs 6 a column. (128 rows through 8192 x 8192: tiles of 128 with K shared 24 us, of 64 37.)
     int64_t best = INT64_MAX;
     for (int tiles_m = (p.M - 1) / tall::MAX_M + 1, tries = 0; tries < 4; tries++, tiles_m++) {
         const int width = ((p.M - 1) / tiles_m + 16) / 16 * 16;
-        const int64_t tiles = (int64_t)((p.M - 1) / width + 1) * q.tiles_n, cost = ((tiles - 1) / sms + 1) * (width > 112 ? width : 112);
+        const int64_t tiles = (int64_t)((p.M - 1) / width + 1) * q.tiles_n;
         if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
-        if (cost < best) best = cost, q.tile_m = width, q.tiles = (int)tiles;
+        int shift = 0;
+        while (shift < 3 && tiles << (shift + 1) <= sms && slabs >= 4 << shift) shift++;
+        const int64_t cost = ((tiles - 1) / sms + 1) * ((slabs - 1 >> shift) + 1) * (width > 112 ? width : 112) + (shift ? 168 + 6 * width : 0);
+        if (cost < best) best = cost, q.tile_m = width, q.tiles = (int)tiles, q.split_shift = shift;
     }
-    const int stage = q.tile_m * tall::TILE_K * 2;
+    const int halves = q.tile_m <= 128 ? 2 : 1, stage = q.tile_m * tall::TILE_K * 2 * halves;
     q.raws = q.tile_m > 160 ? 2 : tall::MAX_RAW;
     q.stages = (tall::SMEM_MOST - 1024 - q.raws * RAW_BYTES) / stage;
-    if (q.stages > tall::MAX_STAGES) q.stages = tall::MAX_STAGES;
+    if (q.stages > tall::MAX_STAGES / halves) q.stages = tall::MAX_STAGES / halves;   // as many as tensor memory has columns for
     const int smem = 1024 + q.raws * RAW_BYTES + q.stages * stage;
-    while (q.split_shift < 3 && q.tiles << (q.split_shift + 1) <= sms && slabs >= 4 << q.split_shift) q.split_shift++;
     const int splits = 1 << q.split_shift;
     CUtensorMap mw, mx;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, tall::SLAB_K / 2, ROWS)) return rc;
     if (const int rc = make_tensor_map(&mx, WHO, MAP_TYPE<T>, p.x, p.M, p.K, p.ldx * 2, tall::TILE_K, q.tile_m)) return rc;
-    constexpr auto kern = tall::matmul_w4_tall<T, FLUSH, ZEROS>;
-    if (const int rc = basalt_k::allow_smem<kern>(WHO, tall::SMEM_MOST)) return rc;
-    return basalt_k::launch_clusters(WHO, kern, splits > 1 || q.tiles < sms ? q.tiles * splits : sms, tall::TALL_THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales,
-                                     p.zeros, (T*)p.c, p.ldc, q, p.status);
+    const auto go = [&](auto two) {
+        constexpr auto kern = tall::matmul_w4_tall<T, FLUSH, ZEROS, decltype(two)::value>;
+        if (const int rc = basalt_k::allow_smem<kern>(WHO, tall::SMEM_MOST)) return rc;
+        return basalt_k::launch_clusters(WHO, kern, splits > 1 || q.tiles < sms ? q.tiles * splits : sms, tall::TALL_THREADS, smem, splits, p.stream, mw, mx, (const T*)p.scales,
+                                         p.zeros, (T*)p.c, p.ldc, q, p.status);
+    };
+    return halves == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
 }
 
 template <class T, int FLUSH, bool ZEROS>
