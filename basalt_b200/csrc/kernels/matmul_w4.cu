@@ -412,7 +412,7 @@ struct Shape {
 };
 
 // HALVES: 64-k tiles in a stage. Two, where the tile is narrow: the thread that issues the MMAs needs some 250 clocks a stage beside them,
-// more than the products of 64 k take there (64 rows, 8192 x 8192: 24.5 us with one, HALVES_HERE with two).
+// more than the products of 64 k take there (64 rows, 8192 x 8192: 24.5 us with one, 22.4 with two).
 template <class T, int FLUSH, bool ZEROS, int HALVES>
 __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                   const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C,
@@ -688,6 +688,14 @@ const char* const WHO = "matmul_w4";
 template <class T>
 constexpr CUtensorMapDataType MAP_TYPE = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 
+// CTAs that share a tile's K, as a power of two, in the kernel for few rows: two fit an SM; split while the tiles leave room and every share
+// keeps two slabs.
+int few_shift(int64_t tiles, int slabs) {
+    int shift = 0;
+    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && slabs >= 4 << shift) shift++;
+    return shift;
+}
+
 template <class T, int NT, int FLUSH, bool ZEROS>
 int launch_few(const Args& p) {
     constexpr int TOKENS = 8 * NT, smem = few::Stage<T, NT, FLUSH, ZEROS>::SMEM;
@@ -695,8 +703,7 @@ int launch_few(const Args& p) {
     if (const int rc = basalt_k::allow_smem<kern>(WHO, smem)) return rc;
     const int tiles_n = (p.N - 1) / ROWS + 1, slabs = (p.K - 1) / few::SLAB_K + 1, groups = (p.K - 1) / p.group + 1;
     const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TOKENS + 1);
-    int shift = 0;   // two CTAs fit an SM: split K while the tiles leave room and every share keeps two slabs
-    while (shift < 3 && tiles << (shift + 1) <= 2 * basalt_k::sm_count() && slabs >= 4 << shift) shift++;
+    const int shift = few_shift(tiles, slabs);
     CUtensorMap mw, mx;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, few::SLAB_K / 2, ROWS)) return rc;
     // one launch takes 65535 tiles of rows of X
@@ -712,25 +719,34 @@ int launch_few(const Args& p) {
     return 0;
 }
 
-template <class T, int FLUSH, bool ZEROS>
-int launch_tall(const Args& p) {
-    constexpr int RAW_BYTES = tall::PACKED_BYTES + SlabScales<T, FLUSH, ZEROS>::BYTES;
-    const int sms = basalt_k::sm_count(), slabs = (p.K - 1) / tall::SLAB_K + 1;
-    tall::Shape q = {p.M, p.N, p.K, p.group, 0, (p.N - 1) / ROWS + 1, 0, 0, 0, (p.K - 1) / p.group + 1, 0, 0};
-    q.aligned = SlabScales<T, FLUSH, ZEROS>::aligned(p.scales, p.zeros, p.group, q.groups);
-    // The width of a tile and the CTAs that share its K (one CTA fits an SM): of the few counts of tiles over M that come near
-    // 256 columns each, the one that costs least. A slab costs what its products do, two clocks a column and 64 k, and not less than
-    // its unpacking, about 112 columns' worth; a join costs 6 a column. (128 rows through 8192 x 8192: tiles of 128 with K shared 24 us, of 64 37.)
-    int64_t best = INT64_MAX;
-    for (int tiles_m = (p.M - 1) / tall::MAX_M + 1, tries = 0; tries < 4; tries++, tiles_m++) {
-        const int width = ((p.M - 1) / tiles_m + 16) / 16 * 16;
-        const int64_t tiles = (int64_t)((p.M - 1) / width + 1) * q.tiles_n;
-        if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
+// The width of a tile of the tcgen05 kernel and the CTAs that share its K (one CTA fits an SM): of the few counts of tiles over M that come near
+// 256 columns each, the one that costs least. A slab costs what its products do, two clocks a column and 64 k, and not less than
+// its unpacking, about 112 columns' worth. (128 rows through 8192 x 8192: tiles of 128 with K shared 24.5 us, of 64 without 37.)
+struct TallPlan {
+    int width, tiles, shift;
+    double time;   // us
+};
+TallPlan plan_tall(int M, int N, int K) {
+    const int sms = basalt_k::sm_count(), slabs = (K - 1) / tall::SLAB_K + 1;
+    TallPlan best = {0, 0, 0, 1e300};
+    for (int tiles_m = (M - 1) / tall::MAX_M + 1, tries = 0; tries < 4; tries++, tiles_m++) {
+        const int width = ((M - 1) / tiles_m + 16) / 16 * 16;
+        const int64_t tiles = (int64_t)((M - 1) / width + 1) * ((N - 1) / ROWS + 1);
+        if (tiles > INT32_MAX / 2) continue;
         int shift = 0;
         while (shift < 3 && tiles << (shift + 1) <= sms && slabs >= 4 << shift) shift++;
-        const int64_t cost = ((tiles - 1) / sms + 1) * ((slabs - 1 >> shift) + 1) * (width > 112 ? width : 112) + (shift ? 168 + 6 * width : 0);
-        if (cost < best) best = cost, q.tile_m = width, q.tiles = (int)tiles, q.split_shift = shift;
+        const double units = (double)((tiles - 1) / sms + 1) * ((slabs - 1 >> shift) + 1) * (width > 112 ? width : 112);
+        const double time = 6.5 + 0.9 / 112 * units + (shift ? 0.5 * (1 << shift) : 0.0);
+        if (time < best.time) best = {width, (int)tiles, shift, time};
     }
+    return best;
+}
+
+template <class T, int FLUSH, bool ZEROS>
+int launch_tall(const Args& p, const TallPlan& plan) {
+    constexpr int RAW_BYTES = tall::PACKED_BYTES + SlabScales<T, FLUSH, ZEROS>::BYTES;
+    const int sms = basalt_k::sm_count(), groups = (p.K - 1) / p.group + 1;
+    tall::Shape q = {p.M, p.N, p.K, p.group, plan.width, (p.N - 1) / ROWS + 1, plan.tiles, 0, 0, groups, plan.shift, SlabScales<T, FLUSH, ZEROS>::aligned(p.scales, p.zeros, p.group, groups)};
     const int halves = q.tile_m <= 128 ? 2 : 1, stage = q.tile_m * tall::TILE_K * 2 * halves;
     q.raws = q.tile_m > 160 ? 2 : tall::MAX_RAW;
     q.stages = (tall::SMEM_MOST - 1024 - q.raws * RAW_BYTES) / stage;
@@ -749,10 +765,21 @@ int launch_tall(const Args& p) {
     return halves == 2 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
 }
 
+// Up to 16 rows go through the kernel for few rows. More do so in tiles of 16, where that is the shorter way: 2.5 us and 1.6 a slab and
+// round of CTAs against the estimate above. (Tiles of 16 / tcgen05, measured: 48 rows, 4096 -> 1024: 6.9 / 8.9 us; 64 rows, 4096 -> 4096:
+// 13.7 / 10.0; 17 rows, 8192 -> 8192: 23.7 / 21.0.) Under 128 rows of weights most of the tcgen05 kernel's lanes would idle.
 template <class T, int FLUSH, bool ZEROS>
 int launch_rows(const Args& p) {
-    if (p.M > 16 && p.N >= ROWS) return launch_tall<T, FLUSH, ZEROS>(p);
-    return p.M <= 8 ? launch_few<T, 1, FLUSH, ZEROS>(p) : launch_few<T, 2, FLUSH, ZEROS>(p);
+    if (p.M <= 8) return launch_few<T, 1, FLUSH, ZEROS>(p);
+    if (p.M > 16 && p.N >= ROWS) {
+        const int slabs = (p.K - 1) / few::SLAB_K + 1;
+        const int64_t tiles = (int64_t)((p.M - 1) / 16 + 1) * ((p.N - 1) / ROWS + 1);
+        const int shift = few_shift(tiles, slabs);
+        const TallPlan plan = plan_tall(p.M, p.N, p.K);
+        if (!plan.tiles) return basalt_k::record_msg(1, WHO, "M * N is too large");
+        if (plan.time < 2.5 + 1.6 * (double)(((tiles << shift) - 1) / (2 * basalt_k::sm_count()) + 1) * ((slabs - 1 >> shift) + 1)) return launch_tall<T, FLUSH, ZEROS>(p, plan);
+    }
+    return launch_few<T, 2, FLUSH, ZEROS>(p);
 }
 
 template <class T, int FLUSH>

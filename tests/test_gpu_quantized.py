@@ -260,7 +260,10 @@ def w4_weights(g, N, K, group, zeros, t, exact):
 
 
 W4_SHAPES = [(1, 1, 1, 32), (1, 128, 256, 128), (2, 127, 33, 32), (8, 130, 255, 64), (9, 64, 257, 128), (16, 300, 1000, 32), (17, 129, 512, 96), (32, 200, 2048, 128), (33, 140, 300, 64),
-             (70, 260, 640, 128), (129, 128, 384, 1024), (200, 300, 1111, 128), (1, 500, 8192, 128), (3, 96, 4096, 64), (1, 140, 16000, 32), (2, 20000, 4500, 128), (13, 19000, 4100, 64), (20, 260, 17000, 96), (31, 20000, 2200, 32), (9, 7000, 129, 128), (5, 129, 2560, 256), (40, 300, 2816, 256), (6, 131, 2048, 64), (70, 130, 4096, 32), (3, 128, 1024, 192)]
+             (70, 260, 640, 128), (129, 128, 384, 1024), (200, 300, 1111, 128), (1, 500, 8192, 128), (3, 96, 4096, 64), (1, 140, 16000, 32), (2, 20000, 4500, 128), (13, 19000, 4100, 64), (20, 260, 17000, 96), (31, 20000, 2200, 32), (9, 7000, 129, 128), (5, 129, 2560, 256), (40, 300, 2816, 256), (6, 131, 2048, 64), (70, 130, 4096, 32), (3, 128, 1024, 192),
+             # the tcgen05 kernel: wide and narrow tiles, one tile and several a CTA, K whole and shared by two, four and eight
+             (520, 4100, 70, 32), (520, 9000, 130, 64), (520, 2100, 777, 96), (400, 520, 8200, 128), (100, 19000, 64, 64), (520, 520, 1111, 128), (700, 130, 3001, 192), (700, 130, 4100, 32),
+             (300, 3000, 1400, 256), (2000, 260, 600, 64)]
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])
@@ -278,7 +281,7 @@ def test_matmul_w4_exact_on_small_integers(gpu, shape, zeros, t):
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])
-@pytest.mark.parametrize("shape", [(1, 300, 4096, 128), (13, 129, 777, 32), (16, 260, 1500, 96), (25, 140, 600, 64), (40, 257, 2049, 64), (150, 100, 900, 64), (300, 384, 1024, 128)])
+@pytest.mark.parametrize("shape", [(1, 300, 4096, 128), (13, 129, 777, 32), (16, 260, 1500, 96), (25, 140, 600, 64), (40, 257, 2049, 64), (150, 100, 900, 64), (300, 384, 1024, 128), (520, 520, 1111, 64), (400, 520, 8200, 128), (100, 19000, 65, 32)])
 def test_matmul_w4_random(gpu, shape, t):
     M, N, K, group = shape
     g = gen(K)
