@@ -176,10 +176,10 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
 //
 // Rows of A (tokens) along the accumulator's lanes. CTA r of the pair loads rows 128 r .. of the tile's A and columns 128 r .. of its
 // B, 32 KB a slab of 128 bytes of K, and holds its 128 rows of the accumulator; the even CTA issues every
-// MMA. Persistent: one warp feeds the ring, one issues, four drain the accumulator of the tile before (two of them
+// MMA, two slabs for each wait (one: 443 us where two take 413, 8192^3 under the power cap; the tensor cores run dry over a wait). Persistent: one warp feeds the ring, one issues, four drain the accumulator of the tile before (two of them
 // in tensor memory), so the stores of a tile hide behind the next one's products.
 namespace pair {
-constexpr int TM = 256, TN = 256, HALF = 128, STAGES = 6, STAGE_BYTES = 2 * HALF * BK, PIECE_BYTES = 32 * 128, PAIR_THREADS = 192, GROUP_M = 8;
+constexpr int TM = 256, TN = 256, HALF = 128, SLABS = 2, STAGES = 3, SLAB_BYTES = 2 * HALF * BK, STAGE_BYTES = SLABS * SLAB_BYTES, PIECE_BYTES = 32 * 128, PAIR_THREADS = 192, GROUP_M = 8;
 constexpr int SMEM = STAGES * STAGE_BYTES + 4 * (PIECE_BYTES + TN * 4) + 1024;
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int tiles_m = (M - 1) / TM + 1, tiles_n = (N - 1) / TN + 1, num_tiles = tiles_m * tiles_n, slabs = (K - 1) / BK + 1;
+    const int tiles_m = (M - 1) / TM + 1, tiles_n = (N - 1) / TN + 1, num_tiles = tiles_m * tiles_n, steps = (K - 1) / (BK * SLABS) + 1;
 
     if (threadIdx.x == 0) {
         gave_up = 0;
@@ -239,13 +239,16 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 int mi, ni;
                 tile_at(t, tiles_m, tiles_n, &mi, &ni);
                 const int m0 = mi * TM + (int)rank * HALF, n0 = ni * TN + (int)rank * HALF;
-                for (int kb = 0; kb < slabs; kb++) {
+                for (int kb = 0; kb < steps; kb++) {
                     ok &= mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, &gave_up);
                     if (!ok) break;
                     const uint32_t fb_local = smem_u32(&full_bar[s]), fb = map_to_cta(fb_local, 0), a_dst = tiles + s * STAGE_BYTES;
                     if (leader) mbar_expect_tx(fb_local, 2 * STAGE_BYTES);
-                    tma_load_2d_pair(a_dst, &map_a, fb, kb * BK, m0);
-                    tma_load_2d_pair(a_dst + HALF * BK, &map_b, fb, kb * BK, n0);
+#pragma unroll
+                    for (int h = 0; h < SLABS; h++) {   // a slab behind the end of K arrives as zeros
+                        tma_load_2d_pair(a_dst + h * SLAB_BYTES, &map_a, fb, (kb * SLABS + h) * BK, m0);
+                        tma_load_2d_pair(a_dst + h * SLAB_BYTES + HALF * BK, &map_b, fb, (kb * SLABS + h) * BK, n0);
+                    }
                     if (++s == STAGES) s = 0, ph ^= 1;
                 }
             }
@@ -263,14 +266,17 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 ok &= mbar_wait(smem_u32(&tempty_bar[buf]), (use & 1) ^ 1, &gave_up);   // both epilogues have drained this accumulator
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int kb = 0; kb < slabs; kb++) {
+                for (int kb = 0; kb < steps; kb++) {
                     ok &= mbar_wait(smem_u32(&full_bar[s]), ph, &gave_up);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t a_src = tiles + s * STAGE_BYTES;
                     const uint64_t da = smem_desc(a_src, 16, 1024), db = smem_desc(a_src + HALF * BK, 16, 1024);
 #pragma unroll
-                    for (int k = 0; k < BK / MMA_K; k++) umma_f8_pair(tmem_base + buf * TN, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (kb | k) != 0);
+                    for (int h = 0; h < SLABS; h++)
+#pragma unroll
+                        for (int k = 0; k < BK / MMA_K; k++)
+                            umma_f8_pair(tmem_base + buf * TN, da + (uint64_t)(h * (SLAB_BYTES >> 4) + 2 * k), db + (uint64_t)(h * (SLAB_BYTES >> 4) + 2 * k), idesc, (kb | h | k) != 0);
                     umma_commit_pair(smem_u32(&empty_bar[s]));
                     if (++s == STAGES) s = 0, ph ^= 1;
                 }

@@ -411,8 +411,9 @@ struct Shape {
     int M, N, K, group, tile_m, tiles_n, tiles, stages, raws, groups, split_shift, aligned;
 };
 
-// HALVES: 64-k tiles in a stage. Two, where the tile is narrow: the thread that issues the MMAs needs some 250 clocks a stage beside them,
-// more than the products of 64 k take there (64 rows, 8192 x 8192: 24.5 us with one, 22.4 with two).
+// HALVES: 64-k tiles in a stage. Two, wherever three such stages fit (tiles of up to 240 columns): the tensor cores run dry while the
+// issuing thread waits for a stage and its barrier's answer, some 250 clocks (64 rows, 8192 x 8192: 24.5 us with one, 22.4 with two; 2048
+// rows, 11008 -> 4096, under the power cap: 170 and 156).
 template <class T, int FLUSH, bool ZEROS, int HALVES>
 __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                   const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C,
@@ -747,7 +748,7 @@ int launch_tall(const Args& p, const TallPlan& plan) {
     constexpr int RAW_BYTES = tall::PACKED_BYTES + SlabScales<T, FLUSH, ZEROS>::BYTES;
     const int sms = basalt_k::sm_count(), groups = (p.K - 1) / p.group + 1;
     tall::Shape q = {p.M, p.N, p.K, p.group, plan.width, (p.N - 1) / ROWS + 1, plan.tiles, 0, 0, groups, plan.shift, SlabScales<T, FLUSH, ZEROS>::aligned(p.scales, p.zeros, p.group, groups)};
-    const int halves = q.tile_m <= 128 ? 2 : 1, stage = q.tile_m * tall::TILE_K * 2 * halves;
+    const int halves = q.tile_m <= 240 ? 2 : 1, stage = q.tile_m * tall::TILE_K * 2 * halves;
     q.raws = q.tile_m > 160 ? 2 : tall::MAX_RAW;
     q.stages = (tall::SMEM_MOST - 1024 - q.raws * RAW_BYTES) / stage;
     if (q.stages > tall::MAX_STAGES / halves) q.stages = tall::MAX_STAGES / halves;   // as many as tensor memory has columns for
