@@ -10,8 +10,12 @@
 // stages (128 bytes of K each) by bulk-tensor loads, thread 0 of warp 1 issues the MMAs, and all four warps drain
 // the accumulator. Where there are fewer tiles than the GPU has room for, a cluster of up to eight
 // CTAs shares one tile, each taking a run of K slabs: the partial sums meet in distributed shared memory and are added in
-// the order of the CTAs, so the result depends on no race and needs no workspace.
+// the order of the CTAs, so the result depends on no race and needs no workspace. (Two such CTAs fit an SM, and their tensor memory,
+// 256 columns at most, with them; no CTA that waits for its cluster can be kept from starting by another's.)
 // Ragged edges are the tensor maps' business: what lies outside a matrix is read as zero.
+// What bounds it: for one row the weights, 14.9 us for 8192 x 8192 (4.5 TB/s; a plain stream of as many bytes takes 11.4 to 12.3, the rest is the
+// way of the first and the last slab); for many rows see the pairs of CTAs below, 8192^3 in 375 us in a burst (2.9 PFLOP/s) and 413 to 430 at the 1.25 GHz
+// that the power cap leaves.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -93,9 +97,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
     wait_for_predecessor();
     if (threadIdx.x == 0 && status && *reinterpret_cast<volatile int32_t*>(status) != 0) gave_up = 1;   // an earlier CTA gave up: do not pile on
     bool ok = true;
-    for (int m = threadIdx.x; m < TN; m += THREADS) scale[m] = m0 + m < M ? a_scales[m0 + m] : 0.0f;
     const float b_scale = n0 + (int)threadIdx.x < N ? b_scales[n0 + threadIdx.x] : 0.0f;
-    __syncthreads();
 
     if (warp == 0 && lane == 0) {
         for (int i = 0; i < count; i++) {
@@ -126,8 +128,14 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
             umma_commit(smem_u32(&empty_bar[s]));
         }
         umma_commit(smem_u32(&acc_bar));
+        if (!ok) {   // let the products already issued end before tensor memory is given back
+            const uint64_t t0 = global_ns();
+            while (global_ns() - t0 < 2000000ull) {}
+        }
+    } else if (warp >= 2) {
+        for (int m = threadIdx.x - 64; m < TN; m += 64) scale[m] = m0 + m < M ? a_scales[m0 + m] : 0.0f;
     }
-    __syncwarp();
+    __syncthreads();
 
     ok &= mbar_wait(smem_u32(&acc_bar), 0, &gave_up);   // on give-up the drain still runs (warp-uniformly) on whatever TMEM holds
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -281,6 +289,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                     if (++s == STAGES) s = 0, ph ^= 1;
                 }
                 umma_commit_pair(smem_u32(&tfull_bar[buf]));
+            }
+            if (!ok) {   // let the products already issued end before tensor memory is given back
+                const uint64_t t0 = global_ns();
+                while (global_ns() - t0 < 2000000ull) {}
             }
         }
     } else {

@@ -1,21 +1,12 @@
-// Product with 4-bit weights for sm_100a, for the few rows of a decode step:
+// Product with 4-bit weights for sm_100a:
 //
 //   C[m, n] = sum_k X[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]
 //
 // X [M x K] and C [M x N] are f16 or bf16; q is four bits, two to a byte along k (even k in the low half); s has X's type,
-// z is an integer (8 where none are given). The weights are read once for all rows of X, and they are what the call
-// costs: N K / 2 bytes.
-//
-// The sum runs on the tensor cores with exact operands: q - z is a small integer, exact in f16 and in bf16, so
-// mma.sync m16n8k16 adds (q - z) * x over a group in f32 and the group's scale multiplies that sum in f32. Nothing but C
-// is rounded to 16 bits. The instruction's order of k is free as long as both operands share it; it is chosen so that one
-// 32-bit word of packed weights (eight k) and one 16-byte load of X (eight k) feed two instructions without a shuffle
-// between threads. (tcgen05.mma would want the unpacked weights back in shared memory: four times the bytes
-// of the packed ones, for at most 32 columns of work.)
-//
-// A CTA takes 128 rows of the weights over its share of K: one warp feeds a ring of stages (256 k) by bulk-tensor loads,
-// eight warps compute (32 rows x half a stage each). A cluster of up to eight CTAs shares a tile's K where tiles are
-// few; the partial sums meet in distributed shared memory and are added in a fixed order.
+// z is an integer (8 where none are given). Two kernels: few rows of X are bound by reading (and unpacking) N K / 2 bytes of weights, many rows by
+// the products. Both read the weights once for a tile of rows, unpack them by putting four bits into the mantissa
+// of a power of two and subtracting, exactly, and add in f32. A cluster of up to eight CTAs shares a tile's K where tiles are few; the
+// partial sums meet in distributed shared memory and are added in a fixed order: no workspace, no atomics, the same bits every time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -191,7 +182,15 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 // ---- few rows of X ----
 //
 // A CTA takes 128 rows of the weights over its share of K: one warp feeds a ring of stages (256 k) by bulk-tensor loads, eight
-// warps compute, 32 rows x half a stage each.
+// warps compute, 32 rows x half a stage each. Operands are exact: q - z is a small integer, exact in f16 and in bf16, so
+// mma.sync m16n8k16 adds (q - z) * x over a group in f32 and the group's scale multiplies that sum in f32. Nothing but C is
+// rounded to 16 bits. The instruction's order of k is free as long as both operands share it; it is chosen so that one
+// 32-bit word of packed weights (eight k) and one 16-byte load of X (eight k) feed two instructions without a shuffle
+// between threads. (tcgen05.mma would save the products, which are not what bounds this: its instructions are 128 rows high, and
+// a group's sum would have to leave tensor memory before its scale.)
+// What bounds it: logic operations, half a warp a clock. Unpacking eight weights takes five of them (seven in bf16), a tile's
+// share of ordering X one more, 7 us of the 11.4 that one row through 8192 x 8192 takes (2.9 TB/s of packed weights; a plain stream of as many bytes
+// takes 6.5). 16 rows, 4096 -> 14336 in groups of 64 with zero points, bf16: 18.2 us.
 namespace few {
 constexpr int SLAB_K = 256, W_BYTES = ROWS * SLAB_K / 2, CONSUMERS = 8, THREADS = 32 * (CONSUMERS + 1), X_BOX_K = 32;
 
@@ -378,15 +377,18 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 }
 }  // namespace few
 
-// ---- many rows of X: the weights unpacked into shared memory for tcgen05.mma ----
+// ---- many rows of X: the weights unpacked into tensor memory for tcgen05.mma ----
 //
 // The weights lie along the accumulator's 128 lanes and up to 256 rows of X along its columns (the width of a tile is the
-// host's choice, a multiple of 16). Teams of four warps turn the 4 KB of packed weights of 64 k into the 16 KB swizzled tile that
-// the MMA reads, (q - z) * s rounded to X's type: unlike the kernel above, which scales sums, this one scales the operand,
-// because a group's sum would have to leave tensor memory for every group. That is one rounding of half a step a weight, of
-// random sign, beside the one of C: the error of C grows by the root of two.
-// Persistent where there are more tiles than SMs (two accumulators: a tile's stores hide behind the next one's products); a
-// cluster shares a tile's K, as above, where there are fewer.
+// host's choice, a multiple of 16). Teams of four warps unpack 64 k each, a thread one row, straight into the tensor memory
+// that the MMA takes its first operand from: (q - z) * s rounded to X's type. Unlike the kernel above, which scales sums, this one
+// scales the operand, because a group's sum would have to leave tensor memory for every group. That is one rounding of half
+// a step a weight, of random sign, beside the one of C: the error of C grows by less than the root of two.
+// (Through shared memory, written once and read by every MMA, the operand made that memory the bound: 2048 rows, 11008 -> 4096, 149 us
+// where this took 122.) Persistent where there are more tiles than SMs; a cluster shares a tile's K where there are fewer.
+// What bounds it: for wide tiles the tensor cores at the clock the power cap leaves (2048 rows, 11008 -> 4096: 1.3 PFLOP/s at 143 us in a burst,
+// 1.18 at 156 in a longer run); for narrow ones the way of a slab from barrier to barrier, some 0.27 us of 64 k (64 rows,
+// 8192 x 8192: 22.4 us, where the weights alone would take 5.3).
 namespace tall {
 constexpr int SLAB_K = 256, TILE_K = 64, PACKED_BYTES = ROWS * SLAB_K / 2, MAX_STAGES = 8, MAX_RAW = 4, MAX_M = 256;
 constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, TEAMS = SLAB_K / TILE_K, TEAM = 4, FIRST_UNPACKER = 4, EPILOGUE = 4;
@@ -542,6 +544,10 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
             }
             umma_commit_elected(smem_u32(&tfull_bar[buf]));
             if (++buf == (uint32_t)accs) buf = 0, use++;
+        }
+        if (!ok) {   // let the products already issued end before tensor memory is given back
+            const uint64_t t0 = global_ns();
+            while (global_ns() - t0 < 2000000ull) {}
         }
     } else if (warp >= FIRST_UNPACKER && warp < FIRST_EPILOGUE) {
         // Four teams of four warps take the four tiles of a slab of packed weights, so that each has four tiles' time for
@@ -752,7 +758,9 @@ int launch_tall(const Args& p, const TallPlan& plan) {
     q.raws = q.tile_m > 160 ? 2 : tall::MAX_RAW;
     q.stages = (tall::SMEM_MOST - 1024 - q.raws * RAW_BYTES) / stage;
     if (q.stages > tall::MAX_STAGES / halves) q.stages = tall::MAX_STAGES / halves;   // as many as tensor memory has columns for
-    const int smem = 1024 + q.raws * RAW_BYTES + q.stages * stage;
+    // The whole SM's shared memory is asked for, used or not. The kernel takes all of the SM's tensor memory, and its clusters' CTAs wait for
+    // one another: beside a kernel of another stream that does the same, each could hold what the other's CTA waits for.
+    const int smem = tall::SMEM_MOST;
     const int splits = 1 << q.split_shift;
     CUtensorMap mw, mx;
     if (const int rc = make_tensor_map(&mw, WHO, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.N, ((int64_t)p.K + 1) / 2, p.ldw, tall::SLAB_K / 2, ROWS)) return rc;
