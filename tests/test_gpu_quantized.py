@@ -356,19 +356,21 @@ def test_a_layer_of_them(gpu, rows_n):
     assert ((got["c4"].double() - want).abs() <= want.abs() * (half * (1 + 2 ** -7) + 2 * U) + size * (2 * hidden * U + weight)).all()
 
 
-def test_two_streams_at_once_and_again_give_the_same_bits(gpu):
+@pytest.mark.parametrize("size", [(12, 1024, 640), (520, 2048, 1030)])
+def test_two_streams_at_once_and_again_give_the_same_bits(gpu, size):
+    """Also where both products share K among clusters, and one of them takes all tensor memory of its SMs."""
     streams = [gpu.create_stream(), gpu.create_stream()]
-    hosts = [layer_buffers(s, 12, 1024, 640)[0] for s in (1, 2)]
+    hosts = [layer_buffers(s, *size)[0] for s in (1, 2)]
     alone = []
     for h in hosts:
         dev = {k: up(gpu, v) for k, v in h.items()}
-        layer(gpu, dev, 12, 1024, 640)
+        layer(gpu, dev, *size)
         gpu.synchronize()
         alone.append({k: down(dev[k], h[k]) for k in LAYER_OUT})
     devs = [{k: up(gpu, v) for k, v in h.items()} for h in hosts]
     for _ in range(20):
         for d, s in zip(devs, streams):
-            layer(gpu, d, 12, 1024, 640, stream=s)
+            layer(gpu, d, *size, stream=s)
     gpu.synchronize()
     for d, h, want in zip(devs, hosts, alone):
         assert all(torch.equal(down(d[k], h[k]).view(torch.uint8), want[k].view(torch.uint8)) for k in LAYER_OUT)
@@ -395,6 +397,49 @@ def test_captured_into_a_graph_and_replayed_on_new_inputs(gpu):
         layer(gpu, fresh, 12, 1024, 640)
         gpu.synchronize()
         assert all(torch.equal(got[k].view(torch.uint8), down(fresh[k], inputs[k]).view(torch.uint8)) for k in LAYER_OUT)
+
+
+def test_rows_a_gigabyte_apart(gpu):
+    """Offsets past 2^31 elements in every matrix that has a row stride."""
+    ld, n, k, cols = 2**30 + 16, 200, 300, 1000
+    g = gen(11)
+    x, res, w = rows(g, 3, cols, torch.float16), rows(g, 3, cols, torch.float16), rows(g, 1, cols, torch.float16)[0]
+    big = [torch.empty(2 * ld + 4096, dtype=torch.float16, device="cuda") for _ in range(2)]
+    apart = lambda b, r, c, t=torch.float16: b.view(t)[: 2 * ld + c].as_strided((r, c), (ld, 1))  # noqa: E731
+    near = {name: v.cuda() for name, v in (("x", x.contiguous()), ("res", res.contiguous()), ("w", w))}
+    out = {}
+    for far in (False, True):
+        xs = apart(big[0], 3, cols) if far else near["x"]
+        xs.copy_(x)
+        ys = apart(big[1], 3, cols) if far else torch.empty(3, cols, dtype=torch.float16, device="cuda")
+        kernels.rms_norm(xs.data_ptr(), ys.data_ptr(), 3, cols, "f16", weight=near["w"].data_ptr(), residual=near["res"].data_ptr(), ldx=xs.stride(0), ldy=ys.stride(0))
+        out.setdefault("norm", []).append(ys.clone())
+        q = apart(big[1], 3, cols, torch.uint8) if far else torch.empty(3, cols, dtype=torch.uint8, device="cuda")
+        s = torch.empty(3, device="cuda")
+        kernels.quantize_e4m3(xs.data_ptr(), q.data_ptr(), s.data_ptr(), 3, cols, "f16", ldx=xs.stride(0), ldq=q.stride(0))
+        out.setdefault("quantize", []).append(q.clone())
+    a = torch.randint(-3, 4, (3, k), generator=g).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    b = torch.randint(-3, 4, (3, k), generator=g).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    x4, w4 = torch.randint(-3, 4, (3, k), generator=g).half(), torch.randint(0, 256, (3, k // 2), generator=g, dtype=torch.uint8)
+    one = torch.ones(n, device="cuda")
+    s4 = torch.ones(3, 10, dtype=torch.float16, device="cuda")
+    pad = lambda t, to: torch.nn.functional.pad(t, (0, to - t.shape[1])).contiguous().cuda()  # noqa: E731
+    for far in (False, True):
+        aa, bb = (apart(big[0], 3, k, torch.uint8), apart(big[1], 3, k, torch.uint8)) if far else (pad(a, 304), pad(b, 304))
+        aa[:, :k].copy_(a), bb[:, :k].copy_(b)
+        c = torch.empty(3, 3, dtype=torch.float32, device="cuda")
+        kernels.matmul_e4m3(aa.data_ptr(), one.data_ptr(), bb.data_ptr(), one.data_ptr(), c.data_ptr(), 3, 3, k, "f32", lda=aa.stride(0), ldb=bb.stride(0))
+        out.setdefault("e4m3", []).append(c)
+        xx, ww = (apart(big[0], 3, k), apart(big[1], 3, k // 2, torch.uint8)) if far else (pad(x4, 304), pad(w4, 160))
+        xx[:, :k].copy_(x4), ww[:, : k // 2].copy_(w4)
+        c = torch.empty(3, 3, dtype=torch.float16, device="cuda")
+        kernels.matmul_w4(xx.data_ptr(), ww.data_ptr(), s4.data_ptr(), c.data_ptr(), 3, 3, k, 32, "f16", ldx=xx.stride(0), ldw=ww.stride(0))
+        out.setdefault("w4", []).append(c)
+    far_c = apart(big[0], 3, 3)
+    kernels.matmul_w4(pad(x4, 304).data_ptr(), ww.data_ptr(), s4.data_ptr(), far_c.data_ptr(), 3, 3, k, 32, "f16", ldx=304, ldw=ww.stride(0), ldc=ld)
+    out["w4"].append(far_c)
+    for name, got in out.items():
+        assert all(torch.equal(v, got[0]) for v in got[1:]), name
 
 
 def test_pointers_outside_device_memory_are_refused(gpu):
