@@ -9,6 +9,9 @@
 // rounding is monotone (max_k |h_k w_k| * r is exactly max_k |h_k w_k r|), the largest |h_k w_k|. So one pass reads the
 // row, one exchange between the row's threads joins both numbers, and the row is written from registers:
 // every input is read once and every output written once.
+//
+// What bounds it: memory. 8192 x 8192 in f16 with a residual to e4m3: 470 MB in 72.0 us, 6.5 TB/s, what a plain copy reaches; 4096 x 14336 bf16 to
+// e4m3: 176 MB in 29.7 us, 5.9 TB/s. One row of 4096 takes 2.1 us, a launch's time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -153,7 +156,8 @@ __device__ __forceinline__ float magnitude(const uint4& u) {
 
 // Rows whose pointers, strides and width are whole 16-byte vectors, V of them in each thread's registers. Every load of the
 // row is issued before its first use and before any store (an output may be an input's buffer, so the compiler
-// keeps their order): the loads in flight are what the memory is kept busy with. Without a residual the row stays
+// keeps their order): the loads in flight are what the memory is kept busy with (8192 x 8192 with a residual: 102.6 us with the
+// residual's loads between total's stores, 72.0 so). Without a residual the row stays
 // in its own type until it is written; with one, h is kept in f32.
 template <class T, bool NORM, bool RESIDUAL, bool E4M3, int V>
 __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const Rows p) {
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
 }
 
 // Rows that start at no vector boundary, or whose width is no whole number of vectors, up to EACH * 512 elements: a block per
-// row, element by element, one read of the row.
+// row, element by element, one read of the row. Bound by its instructions (1023 x 5003 bf16 to e4m3: 8.7 us, 1.8 TB/s; reading twice 14.3).
 constexpr int EACH = 16;
 template <class T, bool NORM, bool RESIDUAL, bool E4M3>
 __global__ void __launch_bounds__(512) rows_by_element(const Rows p) {
@@ -341,7 +345,8 @@ int launch(const Rows& p, const char* who, cudaStream_t s) {
         return basalt_k::launch_clusters(who, rows_twice<T, NORM, E4M3>, p.rows, 512, 0, 1, s, p);
     }
     // Vectors a thread: one where the rows are few and each should be over soon; four where there are rows for every SM, so that
-    // what a thread spends on joining and on the row's factor is shared by more elements.
+    // what a thread spends on joining and on the row's factor is shared by more elements (8192 x 8192: a thousand threads of one
+    // vector each executed 41 instructions an element and took 105 us, of four 22 and 102, before the loads were put first).
     const bool few = p.rows <= basalt_k::sm_count();
     const int v = vectors <= 1024 && few ? 1 : vectors <= 4 * 512 ? 4 : 8;
     int tpr = (int)((vectors + v - 1) / v);

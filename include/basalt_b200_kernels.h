@@ -1,7 +1,8 @@
 /* Hand-written sm_100a CUDA kernels for the five benchmark workloads: the comparators that every
  * emitted kernel is measured against.  The reference ships no CUDA kernels at all (its .cu files
  * are compiler inputs, tests/kernels/ in the reference project); each entry below names the
- * reference example whose kernel signature and result it reproduces at benchmark scale.
+ * reference example whose kernel signature and result it reproduces at benchmark scale.  At the end,
+ * the operators of a quantised linear layer around the matmul.
  *
  * All pointers are device pointers; `stream` is a cudaStream_t / CUstream (NULL = default
  * stream).  Launches are asynchronous.  Return value: 0, or a cudaError_t / CUresult code
@@ -202,9 +203,11 @@ int basalt_k_matmul_e4m3(const void *A, int64_t lda, const float *a_scales, cons
 /* C[m, n] = sum_k X[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group]: X [M x K] and C [M x N] of `type` (F16 or
  * BF16), W the four-bit q, two to a byte along k (k even in the low half), rows ldw bytes apart; scales s [N x
  * ceil(K / group)] of `type` and zeros z [N x ceil(K / group)] (one byte each, 0 .. 128; NULL: 8 everywhere), both
- * without gaps, from a multiple of 4 bytes.  group is a multiple of 32.  Any M, N, K >= 1 (M or N 0 does nothing); X, W and ldw must be
- * multiples of 16 bytes, ldx of 8 elements.  Sums are f32, C is rounded once.  No workspace, no atomics.  `status` as for
- * basalt_k_matmul_f16. */
+ * without gaps, from a multiple of 4 bytes.  group is a multiple of 32.  Any M, N, K >= 1 (M or N 0 does nothing); X, W and
+ * ldw must be multiples of 16 bytes, ldx of 8 elements.  Sums are f32 and C is rounded once.  Up to 16 rows (M) nothing
+ * else is rounded; beyond, a weight (q - z) * s may be rounded to `type` before the product, which must not overflow it.
+ * Bytes beyond a row's K values are not read; rows and columns beyond M and N are left as they were.  No workspace, no
+ * atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16. */
 int basalt_k_matmul_w4(int type, const void *X, int64_t ldx, const void *W, int64_t ldw, const void *scales,
                        const uint8_t *zeros, int group, void *C, int64_t ldc, int M, int N, int K, int32_t *status,
                        void *stream);

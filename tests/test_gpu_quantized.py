@@ -6,6 +6,7 @@ of K terms costs at most K * u * sum|a b| (every partial sum is below sum|a b|, 
 u of it, twice that where the adder truncates; the products themselves are exact in f32), and three more roundings
 for scales. On top comes half a step of the output's type."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -440,6 +441,28 @@ def test_rows_a_gigabyte_apart(gpu):
     out["w4"].append(far_c)
     for name, got in out.items():
         assert all(torch.equal(v, got[0]) for v in got[1:]), name
+
+
+def test_a_thread_that_has_made_no_call_before(gpu):
+    host, _ = layer_buffers(7, 12, 1024, 640)
+    dev = {k: up(gpu, v) for k, v in host.items()}
+    layer(gpu, dev, 12, 1024, 640)
+    gpu.synchronize()
+    want = {k: down(dev[k], host[k]) for k in LAYER_OUT}
+    fresh, trouble = {k: up(gpu, v) for k, v in host.items()}, []
+
+    def run():
+        try:
+            layer(gpu, fresh, 12, 1024, 640)
+        except Exception as e:
+            trouble.append(e)
+
+    thread = threading.Thread(target=run)
+    thread.start()
+    thread.join()
+    gpu.synchronize()
+    assert not trouble, trouble
+    assert all(torch.equal(down(fresh[k], host[k]).view(torch.uint8), want[k].view(torch.uint8)) for k in LAYER_OUT)
 
 
 def test_pointers_outside_device_memory_are_refused(gpu):
