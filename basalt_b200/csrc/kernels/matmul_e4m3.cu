@@ -13,8 +13,8 @@
 // the order of the CTAs, so the result depends on no race and needs no workspace. (Two such CTAs fit an SM, and their tensor memory,
 // 256 columns at most, with them; no CTA that waits for its cluster can be kept from starting by another's.)
 // Ragged edges are the tensor maps' business: what lies outside a matrix is read as zero.
-// What bounds it: for one row the weights, 14.9 us for 8192 x 8192 (4.5 TB/s; a plain stream of as many bytes takes 11.4 to 12.3, the rest is the
-// way of the first and the last slab); for many rows see the pairs of CTAs below, 8192^3 in 375 us in a burst (2.9 PFLOP/s) and 413 to 430 at the 1.25 GHz
+// What bounds it: for one row the weights, 14.2 us for 8192 x 8192 (4.7 TB/s; a plain stream of as many bytes takes 11.4 to 12.3, the rest is the
+// way of the first and the last slab); for many rows see the pairs of CTAs below, 8192^3 in 362 to 372 us in a burst (3.0 PFLOP/s) and 413 to 441 at the 1.25 GHz
 // that the power cap leaves.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

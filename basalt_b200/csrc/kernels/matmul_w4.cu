@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 // a step a weight, of random sign, beside the one of C: the error of C grows by less than the root of two.
 // (Through shared memory, written once and read by every MMA, the operand made that memory the bound: 2048 rows, 11008 -> 4096, 149 us
 // where this took 122.) Persistent where there are more tiles than SMs; a cluster shares a tile's K where there are fewer.
-// What bounds it: for wide tiles the tensor cores at the clock the power cap leaves (2048 rows, 11008 -> 4096: 1.3 PFLOP/s at 143 us in a burst,
+// What bounds it: for wide tiles the tensor cores at the clock the power cap leaves (2048 rows, 11008 -> 4096: 1.3 PFLOP/s at 138 to 141 us in a burst,
 // 1.18 at 156 in a longer run); for narrow ones the way of a slab from barrier to barrier, some 0.27 us of 64 k (64 rows,
 // 8192 x 8192: 22.4 us, where the weights alone would take 5.3).
 namespace tall {
