@@ -28,6 +28,7 @@ namespace {
 
 constexpr float E4M3_MAX = 448.0f;
 constexpr float SCALE_MIN = 1.17549435e-38f;   // 2^-126: a row of zeros has a scale whose reciprocal is finite
+constexpr float SMALL = 1e-15f;   // 448 / SMALL * r stays below 2^127 while r, which is at most 1 / sqrt(eps), does not exceed 1e20
 
 struct Rows {
     const void *x, *residual, *weight;
@@ -125,19 +126,29 @@ __device__ __forceinline__ void join_row(float& sum, float& top) {
     }
 }
 
-// What the row's outputs are multiplied by, from the joined numbers; the row's first thread stores the scale. The reciprocal
+// What the row's outputs are multiplied by, from the joined numbers, in two factors; the row's first thread stores the scale. The reciprocal
 // square root and the reciprocal are the hardware's (each off by at most two f32 steps, 2^-22 of the value): the exact ones cost every thread
-// more instructions than its elements do.
+// more instructions than its elements do. The second factor is one but for rows so small that the product of both could exceed f32
+// (zeros, first of all, whose r is 1 / sqrt(eps) and whose scale is 2^-126: their bytes are zeros, and 0 * inf is none).
+struct Factor {
+    float first, second;
+};
+__device__ __forceinline__ float operator*(float v, const Factor& f) {
+    v *= f.first;
+    return f.second == 1.0f ? v : v * f.second;   // all threads of a row go one way
+}
 template <bool NORM, bool E4M3>
-__device__ __forceinline__ float row_factor(const Rows& p, int row, bool active, float sum, float top) {
+__device__ __forceinline__ Factor row_factor(const Rows& p, int row, bool active, float sum, float top) {
     const float r = NORM ? rsqrtf(sum * p.per_col + p.eps) : 1.0f;
-    if (!E4M3) return r;
+    if (!E4M3) return {r, 1.0f};
     float most = top * r;
     if (most < E4M3_MAX * SCALE_MIN) most = E4M3_MAX * SCALE_MIN;   // false for a NaN, which stays
     if (active && threadIdx.x == 0) p.scales[row] = most / E4M3_MAX;
     float inverse;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(most));
-    return r * (E4M3_MAX * inverse);
+    inverse *= E4M3_MAX;   // at most 2^126
+    if (NORM && most < SMALL) return {r, inverse};
+    return {r * inverse, 1.0f};
 }
 
 // The largest magnitude in a vector of T; 16-bit values are compared two at a time as they are.
@@ -214,7 +225,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
         }
     }
     join_row(sum, top);
-    const float f = row_factor<NORM, E4M3>(p, row, active, sum, top);
+    const Factor f = row_factor<NORM, E4M3>(p, row, active, sum, top);
 #pragma unroll
     for (int v = 0; v < V; v++) {
         if (threadIdx.x + v * blockDim.x >= vectors) continue;
@@ -230,7 +241,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
             }
         }
 #pragma unroll
-        for (int j = 0; j < W; j++) e[j] *= f;
+        for (int j = 0; j < W; j++) e[j] = e[j] * f;
         const int at = (threadIdx.x + v * blockDim.x) * W;
         if constexpr (E4M3) store_e4m3((uint8_t*)p.y + row * p.ldy + at, e);
         else store_vec((T*)p.y + row * p.ldy + at, e);
@@ -280,7 +291,7 @@ __global__ void __launch_bounds__(512) rows_by_element(const Rows p) {
         if (E4M3) top = max_nan(top, fabsf(h[v]));
     }
     join_row(sum, top);
-    const float f = row_factor<NORM, E4M3>(p, row, true, sum, top);
+    const Factor f = row_factor<NORM, E4M3>(p, row, true, sum, top);
     T* y = (T*)p.y + row * p.ldy + threadIdx.x;
     uint8_t* bytes = (uint8_t*)p.y + row * p.ldy + threadIdx.x;
 #pragma unroll
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
         top = max_nan(top, fabsf(h));
     }
     join_row(sum, top);
-    const float f = row_factor<NORM, E4M3>(p, row, true, sum, top);
+    const Factor f = row_factor<NORM, E4M3>(p, row, true, sum, top);
     for (int64_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
         float h = load_one(x + i);
         if (residual) {

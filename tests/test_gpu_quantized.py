@@ -146,6 +146,30 @@ def test_rows_of_zeros_infinities_and_nans_stay_among_themselves(gpu, cols):
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("cols", [1, 64, 77, 4096, 9001])
+def test_norm_of_rows_that_cancel_or_nearly(gpu, t, cols):
+    """Rows whose sum with the residual is zero (a padded batch), or so small that the norm's factor times the inverse scale exceeds f32: zeros
+    stay zeros, and small values are what the formula says. The small ones are exact in their type, and so are their products with r
+    up to one rounding, because they stay normal numbers of f32."""
+    x = rows(gen(6), 6, cols, T[t])
+    res = torch.zeros_like(x)
+    res[1], x[3], res[4] = -x[1], 0, 1.0
+    x[4] = -1.0
+    if t != "f16":
+        x[2] = torch.randint(1, 4, (cols,), generator=gen(7)).to(T[t]) * 2.0 ** -127
+        x[5] = 2.0 ** -122
+    for residual in (res, None):
+        y, sc, total = torch.full((6, cols), 0x55, dtype=torch.uint8), torch.full((6,), 5.0), torch.zeros(6, cols, dtype=T[t])
+        dy, ds, dx, w = up(gpu, y), up(gpu, sc), up(gpu, x), up(gpu, torch.ones(cols, dtype=T[t]))
+        kernels.rms_norm(dx, dy, 6, cols, t, weight=w, eps=1e-6, residual=None if residual is None else up(gpu, residual), total=None if residual is None else up(gpu, total), scales=ds)
+        gpu.synchronize()
+        _, want = exact_norm(x, residual, torch.ones(cols, dtype=T[t]), 1e-6)
+        check_e4m3(down(dy, y), down(ds, sc), want, (cols / 2 + 10) * U)
+        zero = (want == 0).all(1)
+        assert (down(dy, y)[zero] & 0x7F == 0).all() and (down(ds, sc)[zero] == SCALE_MIN).all() and zero.sum() >= (1 if residual is None else 3)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("pad", [0, 5])
 def test_quantize(gpu, t, pad):
     for i, (n, cols) in enumerate(NORM_SHAPES):
