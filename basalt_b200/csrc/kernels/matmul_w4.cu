@@ -35,7 +35,7 @@ __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // BYTES (4, 8 or 16, and so aligned) from global to shared memory, asynchronously. The first `valid` of them are read (none, if it is
-// negative); the others arrive as zeros.
+// negative; the address has to be aligned all the same); the others arrive as zeros.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, int valid = BYTES) {
     const int n = max(0, min(BYTES, valid));
@@ -60,9 +60,10 @@ struct SlabScales {
 
     // One warp's copies of the rows from n0; lane l has rows l, l + 32, l + 64 and l + 96.
     struct Copies {
-        const uint8_t *scale_row[4], *zero_row[4], *scale_end, *zero_end;
+        const uint8_t *scale_row[4], *zero_row[4], *scale_base, *zero_base, *scale_end, *zero_end;
         __device__ __forceinline__ Copies(const void* scales, const uint8_t* zeros, int n0, int N, int groups, int lane) {
-            scale_end = (const uint8_t*)scales + (int64_t)N * groups * 2, zero_end = zeros + (ZEROS ? (int64_t)N * groups : 0);
+            scale_base = (const uint8_t*)scales, zero_base = zeros;
+            scale_end = scale_base + (int64_t)N * groups * 2, zero_end = zeros + (ZEROS ? (int64_t)N * groups : 0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int64_t first = (int64_t)min(n0 + lane + 32 * r, N - 1) * groups;   // rows past the last get its scales
@@ -86,12 +87,12 @@ struct SlabScales {
 #pragma unroll
                     for (int w = 0; w < SCALE_WORDS; w++) {
                         const bool in = sw + 4 * w < scale_end;
-                        copy_async<4>(at + (row * SCALE_WORDS + w) * 4, in ? sw + 4 * w : scale_row[0], in ? (int)min((int64_t)4, scale_end - sw - 4 * w) : 0);
+                        copy_async<4>(at + (row * SCALE_WORDS + w) * 4, in ? sw + 4 * w : scale_base, in ? (int)min((int64_t)4, scale_end - sw - 4 * w) : 0);
                     }
 #pragma unroll
                     for (int w = 0; w < ZERO_WORDS; w++) {
                         const bool in = zw + 4 * w < zero_end;
-                        copy_async<4>(at + ZERO_AT + (row * ZERO_WORDS + w) * 4, in ? zw + 4 * w : zero_row[0], in ? (int)min((int64_t)4, zero_end - zw - 4 * w) : 0);
+                        copy_async<4>(at + ZERO_AT + (row * ZERO_WORDS + w) * 4, in ? zw + 4 * w : zero_base, in ? (int)min((int64_t)4, zero_end - zw - 4 * w) : 0);
                     }
                 }
             }
