@@ -227,13 +227,15 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) {   // the same warp of both CTAs allocates for the pair
+    __syncthreads();
+    cluster_sync_all();   // the peer runs and its barriers are initialised: only from here on may anything reach into it, and allocating for the pair does
+    if (warp == 1) {      // the same warp of both CTAs
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    cluster_sync_all();   // the peer's barriers are initialised before anything can signal them
+    cluster_sync_all();   // the peer's tensor memory is allocated
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
     wait_for_predecessor();
@@ -366,6 +368,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     cluster_sync_all();   // the peer has stopped naming this CTA's barriers, shared and tensor memory
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    __syncwarp();
+    cluster_sync_all();   // neither leaves while the other still frees the pair's
 }
 }  // namespace pair
 
