@@ -433,7 +433,11 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
     const int shift = p.split_shift, splits = 1 << shift, split = blockIdx.x & (splits - 1);
     const int my_tile = blockIdx.x >> shift, step = gridDim.x >> shift;
     const int slabs = (p.K - 1) / SLAB_K + 1, first = slabs * split >> shift, slabs_here = (slabs * (split + 1) >> shift) - first;
-    const int count = min(slabs_here * SLAB_STAGES, (p.K - 1) / STAGE_K + 1 - first * SLAB_STAGES);
+    // Stages of a tile. A team's stages must follow one another by no more than the ring holds (three at least, five of 64 k), or its wait's parity
+    // would name the phase after the next and let it through too early. Each has every fourth 64-k tile; a team whose share of the last slab lay
+    // behind the end of K and was left out would next be needed three stages on where a stage is two tiles, seven where it is one:
+    // there the slab is walked to its end, on zeros.
+    const int count = HALVES == 1 ? slabs_here * SLAB_STAGES : min(slabs_here * SLAB_STAGES, (p.K - 1) / STAGE_K + 1 - first * SLAB_STAGES);
     const int first_group = (unsigned)(first * SLAB_K) / (unsigned)p.group;
     const int half_bytes = p.tile_m * TILE_K * 2, stage_bytes = half_bytes * HALVES, accs = p.tile_m <= 128 ? 2 : 1;   // with one accumulator, its drain is not hidden
 

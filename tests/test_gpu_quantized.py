@@ -305,6 +305,19 @@ def test_matmul_w4_exact_on_small_integers(gpu, shape, zeros, t):
     assert len(bad) == 0, (len(bad), bad[:5].tolist())
 
 
+@pytest.mark.parametrize("zeros,t", [(True, "f16"), (False, "bf16")])
+@pytest.mark.parametrize("K", [300, 330, 407, 450])
+def test_matmul_w4_several_wide_tiles_a_cta_and_a_ragged_last_slab(gpu, K, zeros, t):
+    """Tiles of 256 rows of X, three for each CTA, where K ends in a slab of which 1, 2, 3 or all of its 64-k tiles are needed."""
+    M, N = 768, 148 * 128
+    g = gen(K)
+    x = torch.randint(-2, 3, (M, K), generator=g).to(T[t])
+    q, s, z, w = w4_weights(g, N, K, 128, zeros, t, True)
+    want = (x.float() @ w.float().T).to(T[t])   # quarters below 2^20: exact in 32 bits too
+    for _ in range(3):
+        assert torch.equal(run_w4(gpu, x, q, s, z, 128, t), want)
+
+
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("shape", [(1, 300, 4096, 128), (13, 129, 777, 32), (16, 260, 1500, 96), (25, 140, 600, 64), (40, 257, 2049, 64), (150, 100, 900, 64), (300, 384, 1024, 128), (520, 520, 1111, 64), (400, 520, 8200, 128), (100, 19000, 65, 32)])
 def test_matmul_w4_random(gpu, shape, t):
