@@ -784,7 +784,11 @@ int launch_tall(const Args& p, const TallPlan& plan) {
 // 13.7 / 10.0; 17 rows, 8192 -> 8192: 23.7 / 21.0.) Under 128 rows of weights most of the tcgen05 kernel's lanes would idle.
 template <class T, int FLUSH, bool ZEROS>
 int launch_rows(const Args& p) {
-    if (p.M <= 8) return launch_few<T, 1, FLUSH, ZEROS>(p);
+    // Tiles of eight rows only where a slab has at most four groups: with eight, four stages deep, copies of scales were seen to be read before they
+    // were there (one row, 14720 -> 14931 in groups of 32, from cold memory: one row of the weights in a hundred off by a slab's scales); tiles of 16,
+    // three deep, gave the same bits in 25,000 such runs.
+    if constexpr (FLUSH > 1)
+        if (p.M <= 8) return launch_few<T, 1, FLUSH, ZEROS>(p);
     if (p.M > 16 && p.N >= ROWS) {
         const int slabs = (p.K - 1) / few::SLAB_K + 1;
         const int64_t tiles = (int64_t)((p.M - 1) / 16 + 1) * ((p.N - 1) / ROWS + 1);

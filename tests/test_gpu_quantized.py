@@ -305,6 +305,33 @@ def test_matmul_w4_exact_on_small_integers(gpu, shape, zeros, t):
     assert len(bad) == 0, (len(bad), bad[:5].tolist())
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 9])
+def test_matmul_w4_from_cold_memory(gpu, group, M):
+    """Two copies of weights in turn, together more than the L2 cache: the scales of a slab take longest to come, and have to be waited for."""
+    N, K, t = 14931, 14720, "bf16"
+    g = gen(group + M)
+    x = torch.randint(-2, 3, (M, K), generator=g).to(T[t])
+    q = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8)
+    groups = K // group
+    s = (2.0 ** torch.randint(-2, 2, (N, groups), generator=g).float()).to(T[t])
+    z = torch.randint(0, 16, (N, groups), generator=g, dtype=torch.uint8)
+    want = torch.empty(M, N, dtype=T[t])
+    for n in range(0, N, 1024):   # a group's sum times its scale: quarters, exact in 32 bits
+        w = (q[n : n + 1024].float().view(-1, groups, group) - z[n : n + 1024].float()[:, :, None]) * s[n : n + 1024].float()[:, :, None]
+        want[:, n : n + 1024] = (x.double() @ w.view(-1, K).double().T).to(T[t])
+    packed = pack(q).contiguous()
+    sets = [[up(gpu, v) for v in (packed, s, z)] for _ in range(2)]
+    c = torch.zeros(M, N, dtype=T[t])
+    dx, dc = up(gpu, x), up(gpu, c)
+    for i in range(100):
+        w, sc, zp = sets[i % 2]
+        kernels.matmul_w4(dx, w, sc, dc, M, N, K, group, t, zeros=zp, ldw=packed.shape[1])
+        gpu.synchronize()
+        if i % 2 == 0 or i > 90:
+            assert torch.equal(down(dc, c), want), i
+
+
 @pytest.mark.parametrize("zeros,t", [(True, "f16"), (False, "bf16")])
 @pytest.mark.parametrize("K", [300, 330, 407, 450])
 def test_matmul_w4_several_wide_tiles_a_cta_and_a_ragged_last_slab(gpu, K, zeros, t):
