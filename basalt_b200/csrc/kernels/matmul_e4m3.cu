@@ -57,10 +57,18 @@ __host__ __device__ constexpr int sums_at() { return TN <= 32 ? ring_of<TN>() : 
 template <int TN>
 __host__ __device__ constexpr int smem_of() { return ring_of<TN>() + (TN <= 32 ? TN * BN * 4 : 0) + 1024; }   // at most 99 KB: two CTAs fit an SM
 
+// C = v, or C += v (f32 alone: a later part of a long K, see launch_type)
+template <class T>
+__device__ __forceinline__ void store_sum(T* c, float v, int add) {
+    if constexpr (sizeof(T) == 4)
+        if (add) v += *c;
+    store_as(c, v);
+}
+
 template <class T, int TN>
 __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
                                                               const float* __restrict__ a_scales, const float* __restrict__ b_scales, T* __restrict__ C,
-                                                              int64_t ldc, int M, int N, int K, int shift, int32_t* status) {
+                                                              int64_t ldc, int M, int N, int K, int shift, int add, int32_t* status) {
     constexpr int STAGES = stages_of<TN>(), A_BYTES = TN * BK, STAGE_BYTES = B_BYTES + A_BYTES;
     constexpr uint32_t TMEM_COLS = TN < 32 ? 32 : TN;
     extern __shared__ uint8_t smem_raw[];
@@ -158,7 +166,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
         } else if (n < N) {
 #pragma unroll
             for (int j = 0; j < 16; j++)
-                if (c + j < tokens) store_as(C + (m0 + c + j) * ldc + n, __uint_as_float(r[j]) * scale[c + j] * b_scale);
+                if (c + j < tokens) store_sum(C + (m0 + c + j) * ldc + n, __uint_as_float(r[j]) * scale[c + j] * b_scale, add);
         }
     }
     if (splits > 1) {
@@ -169,7 +177,7 @@ __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_const
             for (int c = split; c < tokens; c += splits) {
                 float total = 0.0f;
                 for (int q = 0; q < splits; q++) total += sums[(q * each + (c >> shift)) * BN + threadIdx.x];
-                store_as(C + (m0 + c) * ldc + n, total * scale[c] * b_scale);
+                store_sum(C + (m0 + c) * ldc + n, total * scale[c] * b_scale, add);
             }
         }
     }
@@ -202,7 +210,7 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* m,
 template <class T, bool VECTORS>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     matmul_e4m3_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const float* __restrict__ a_scales,
-                     const float* __restrict__ b_scales, T* __restrict__ C, int64_t ldc, int M, int N, int K, int32_t* status) {
+                     const float* __restrict__ b_scales, T* __restrict__ C, int64_t ldc, int M, int N, int K, int add, int32_t* status) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tfull_bar[2], tempty_bar[2];
     __shared__ uint32_t tmem_slot;
@@ -347,8 +355,16 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int m = m0 + 4 * i + row;
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + (4 * i + row) * 128 + ((piece ^ ((4 * i + row) & 7)) << 4));
+                    uint4 v = *reinterpret_cast<const uint4*>(stage + (4 * i + row) * 128 + ((piece ^ ((4 * i + row) & 7)) << 4));
                     T* to = C + m * ldc + n;
+                    if constexpr (sizeof(T) == 4) {
+                        if (add && m < M) {
+                            float* e = reinterpret_cast<float*>(&v);
+#pragma unroll
+                            for (int j = 0; j < W; j++)
+                                if (n + j < N) e[j] += to[j];
+                        }
+                    }
                     if (VECTORS && m < M && n + W <= N) *reinterpret_cast<uint4*>(to) = v;
                     else if (m < M) {
                         const T* e = reinterpret_cast<const T*>(&v);
@@ -378,12 +394,13 @@ struct Args {
     const float *a_scales, *b_scales;
     void* c;
     int64_t lda, ldb, ldc;
-    int M, N, K;
+    int M, N, K, add;
     int32_t* status;
     cudaStream_t stream;
 };
 
 const char* const WHO = "matmul_e4m3";
+constexpr int PART_K = 8192;   // of one launch into an f32 C
 
 // How many CTAs share a tile's K, as a power of two: two CTAs fit an SM; split while the tiles leave room and every share keeps four slabs.
 int split_shift(int64_t tiles, int slabs) {
@@ -404,7 +421,7 @@ int launch(const Args& p) {
     const int64_t tiles = (int64_t)tiles_n * ((p.M - 1) / TN + 1);
     const int shift = split_shift(tiles, slabs);
     const dim3 grid(tiles_n << shift, (p.M - 1) / TN + 1);
-    return basalt_k::launch_clusters(WHO, kern, grid, THREADS, smem, 1 << shift, p.stream, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, shift, p.status);
+    return basalt_k::launch_clusters(WHO, kern, grid, THREADS, smem, 1 << shift, p.stream, mb, ma, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, shift, p.add, p.status);
 }
 
 template <class T, bool VECTORS>
@@ -417,7 +434,7 @@ int launch_pair(const Args& p) {
     const int64_t tiles = (int64_t)((p.M - 1) / pair::TM + 1) * ((p.N - 1) / pair::TN + 1);
     if (tiles > INT32_MAX / 2) return basalt_k::record_msg(1, WHO, "M * N is too large");
     const int pairs = (int)(tiles < basalt_k::sm_count() / 2 ? tiles : basalt_k::sm_count() / 2);
-    return basalt_k::launch_clusters(WHO, kern, 2 * pairs, pair::PAIR_THREADS, pair::SMEM, 2, p.stream, ma, mb, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, p.status);
+    return basalt_k::launch_clusters(WHO, kern, 2 * pairs, pair::PAIR_THREADS, pair::SMEM, 2, p.stream, ma, mb, p.a_scales, p.b_scales, (T*)p.c, p.ldc, p.M, p.N, p.K, p.add, p.status);
 }
 
 // What a call takes, in microseconds, by the kernel above with tiles of TN rows of A: a slab takes a round of CTAs 0.31 to 0.51; the weights
@@ -477,8 +494,16 @@ extern "C" int basalt_k_matmul_e4m3(const void* A, int64_t lda, const float* a_s
     if (overlap(c, {A, M, K, lda, 1}) || overlap(c, {B, N, K, ldb, 1}) || overlap(c, {a_scales, 1, M, M, 4}) || overlap(c, {b_scales, 1, N, N, 4}))
         return basalt_k::record_msg(1, WHO, "C overlaps an input");
     if (const int rc = basalt_k::check_device_pointers(WHO, {A, a_scales, B, b_scales, C, status})) return rc;
-    const Args p = {A, B, a_scales, b_scales, C, lda, ldb, ldc, M, N, K, status, (cudaStream_t)stream};
+    const Args p = {A, B, a_scales, b_scales, C, lda, ldb, ldc, M, N, K, 0, status, (cudaStream_t)stream};
     if (c_type == BASALT_K_TYPE_F16) return launch_type<__half>(p);
     if (c_type == BASALT_K_TYPE_BF16) return launch_type<__nv_bfloat16>(p);
-    return launch_type<float>(p);
+    // The tensor cores' f32 sums are truncated, term by term, which costs some 9e-11 of the result for each k: 1.4e-6 at 16,384. An f32 result
+    // shows it, so K goes in equal parts of at most 8192, each rounded and added to C in turn.
+    const int parts = (K - 1) / PART_K + 1, part = ((K - 1) / parts / BK + 1) * BK;
+    for (int k = 0; k < K; k += part) {
+        Args q = p;
+        q.a = (const uint8_t*)A + k, q.b = (const uint8_t*)B + k, q.K = K - k < part ? K - k : part, q.add = k > 0;
+        if (const int rc = launch_type<float>(q)) return rc;
+    }
+    return 0;
 }

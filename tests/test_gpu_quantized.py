@@ -238,6 +238,19 @@ def test_matmul_e4m3_random(gpu, shape, out):
     assert float((got - want).norm() / want.norm()) <= 0.6 * HALF[out] + 2.0 ** -19   # what errors of random signs leave: a uniform rounding's spread, and 32 u
 
 
+@pytest.mark.parametrize("shape", [(3, 130, 16384), (520, 2600, 16300), (150, 140, 20000), (300, 300, 8193)])
+def test_matmul_e4m3_long_sums_in_f32(gpu, shape):
+    """K in parts of at most 8192, added to C one after the other. The bound is a part's worst: every one of its additions truncated (2 u each)."""
+    M, N, K = shape
+    g = gen(K)
+    qa, qb = e4m3_rows(torch.rand(M, K, generator=g) + 0.5, 0), e4m3_rows(torch.rand(N, K, generator=g) + 0.5, 0)
+    sa, sb = torch.rand(M, generator=g) + 0.5, torch.rand(N, generator=g) + 0.5
+    va, vb = (q.view(torch.float8_e4m3fn).double()[:, :K] for q in (qa, qb))
+    want = (va @ vb.T) * (sa.double()[:, None] * sb.double())
+    got = run_e4m3(gpu, qa, sa, qb, sb, K, "f32").double()
+    assert ((got - want).abs() <= want * (8192 + 4) * 2 * U).all()
+
+
 def test_matmul_e4m3_nan_and_infinite_scales_stay_in_their_rows(gpu):
     a, b = e4m3_rows(torch.ones(20, 64), 0), e4m3_rows(torch.ones(140, 64), 0)
     a[3, 10], b[130, 5] = 0x7F, 0xFF
