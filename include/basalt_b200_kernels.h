@@ -195,7 +195,8 @@ int basalt_k_quantize_e4m3(int type, const void *x, int64_t ldx, void *q, int64_
  * channel) are e4m3, the sums f32 on tcgen05 tensor cores, C [M x N] is of c_type (F16, BF16, F32), rounded once.  Any M, N, K >= 1
  * (M or N 0 does nothing); A, B, lda and ldb must be multiples of 16 bytes (pad the rows: bytes
  * beyond K are not read), C and ldc need their element's alignment only.  Rows and columns beyond M and N are left as
- * they were.  No workspace, no atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16. */
+ * they were.  No workspace, no atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16.
+ * Into f32, a K beyond 8192 goes in several launches whose results are added to C in turn. */
 int basalt_k_matmul_e4m3(const void *A, int64_t lda, const float *a_scales, const void *B, int64_t ldb,
                          const float *b_scales, int c_type, void *C, int64_t ldc, int M, int N, int K, int32_t *status,
                          void *stream);
