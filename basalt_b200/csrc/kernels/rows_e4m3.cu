@@ -127,8 +127,8 @@ __device__ __forceinline__ void join_row(float& sum, float& top) {
 }
 
 // What the row's outputs are multiplied by, from the joined numbers, in two factors; the row's first thread stores the scale. The reciprocal
-// square root and the reciprocal are the hardware's (each off by at most two f32 steps, 2^-22 of the value): the exact ones cost every thread
-// more instructions than its elements do. The second factor is one but for rows so small that the product of both could exceed f32
+// square root is the hardware's, off by at most two f32 steps, 2^-22 of the value. The reciprocal is that of the scale, which lies between 2^-126 and
+// 2^119.2: the row's maximum goes up to 2^128, and the reciprocal of one above 2^126 would be subnormal. The second factor is one but for rows so small that the product of both could exceed f32
 // (zeros, first of all, whose r is 1 / sqrt(eps) and whose scale is 2^-126: their bytes are zeros, and 0 * inf is none).
 struct Factor {
     float first, second;
@@ -144,9 +144,7 @@ __device__ __forceinline__ Factor row_factor(const Rows& p, int row, bool active
     float most = top * r;
     if (most < E4M3_MAX * SCALE_MIN) most = E4M3_MAX * SCALE_MIN;   // false for a NaN, which stays
     if (active && threadIdx.x == 0) p.scales[row] = most / E4M3_MAX;
-    float inverse;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(most));
-    inverse *= E4M3_MAX;   // at most 2^126
+    const float inverse = __frcp_rn(most / E4M3_MAX);   // of the scale: the maximum's own would be a subnormal number above 2^126
     if (NORM && most < SMALL) return {r, inverse};
     return {r * inverse, 1.0f};
 }
