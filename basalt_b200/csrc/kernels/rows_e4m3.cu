@@ -3,7 +3,7 @@
 //
 //   h = x + residual                              (f32)          total = h rounded to the rows' type
 //   y = h * w / sqrt(mean(h^2) + eps)             (f32)
-//   s = max(max_k |y_k| / 448, 2^-126)            one per row    q = y / s rounded to e4m3
+//   s = max(max_k |y_k| / 448, 2^-126)            one per row    q = y / s (f32) rounded to e4m3
 //
 // Both need one number of the whole row before the first output: the sum of squares and, because
 // rounding is monotone (max_k |h_k w_k| * r is exactly max_k |h_k w_k r|), the largest |h_k w_k|. So one pass reads the
@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -28,15 +29,13 @@ namespace {
 
 constexpr float E4M3_MAX = 448.0f;
 constexpr float SCALE_MIN = 1.17549435e-38f;   // 2^-126: a row of zeros has a scale whose reciprocal is finite
-constexpr float SMALL = 1e-15f;   // 448 / SMALL * r stays below 2^127 while r, which is at most 1 / sqrt(eps), does not exceed 1e20
 
 struct Rows {
     const void *x, *residual, *weight;
     void *total, *y;
     float* scales;
-    int64_t ldx, ldr, ldt, ldy;
-    int rows, cols;
-    float eps, per_col;   // per_col: 1 / cols
+    int ldx, ldr, ldt, ldy, rows, cols;   // (88 bytes of parameters; with 64-bit strides a launch took the host 0.3 us longer)
+    float eps, per_col_high, per_col_low;   // 1 / cols, as a sum of two
 };
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -87,6 +86,18 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC<T>]) {
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
+// Two f32 in a 64-bit register, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t two(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
 __device__ __forceinline__ uint32_t four_e4m3(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
@@ -97,6 +108,7 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&f)[N]) {
     if constexpr (N == 4) *reinterpret_cast<uint32_t*>(p) = four_e4m3(f[0], f[1], f[2], f[3]);
     else *reinterpret_cast<uint2*>(p) = make_uint2(four_e4m3(f[0], f[1], f[2], f[3]), four_e4m3(f[4], f[5], f[6], f[7]));
 }
+__device__ __forceinline__ uint8_t one_e4m3(float f) { return (uint8_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3); }
 
 // The larger of two, NaN where either is: a NaN in a row reaches the row's scale instead of vanishing in it.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -126,27 +138,69 @@ __device__ __forceinline__ void join_row(float& sum, float& top) {
     }
 }
 
-// What the row's outputs are multiplied by, from the joined numbers, in two factors; the row's first thread stores the scale. The reciprocal
-// square root is the hardware's, off by at most two f32 steps, 2^-22 of the value. The reciprocal is that of the scale, which lies between 2^-126 and
-// 2^119.2: the row's maximum goes up to 2^128, and the reciprocal of one above 2^126 would be subnormal. The second factor is one but for rows so small that the product of both could exceed f32
-// (zeros, first of all, whose r is 1 / sqrt(eps) and whose scale is 2^-126: their bytes are zeros, and 0 * inf is none).
-struct Factor {
-    float first, second;
-};
-__device__ __forceinline__ float operator*(float v, const Factor& f) {
-    v *= f.first;
-    return f.second == 1.0f ? v : v * f.second;   // all threads of a row go one way
-}
+// What the joined numbers make of a row's values: y = v * r and, for e4m3, y / scale = v * (r / scale). The row's first thread stores the scale.
+//
+// The quotient is the f32 one by the stored scale, so that a y half-way between two e4m3 numbers is rounded as a tie, which a product with a
+// rounded reciprocal is not (8 bits of x over 8 bits of the maximum meet ties often: 8 bytes in 10,000 of bf16 rows went to the other neighbour).
+// A division each would cost more than everything else that is done for an element. So r / scale is kept as a sum of two f32,
+// high + low, that is off by 2^-45 of it (2^-30 where the row's largest number lies near f32's, because low is subnormal then), and
+// v * high + (v * low) is one product and one fused multiply-add, rounded once: a quotient that f32 holds is exact, and no other is off by more than half a step
+// and 2^-30 of it. `high` lies a little below, so that `low` is positive and a zero keeps its sign.
+// (Calls behind one another, so / with the product alone: 4096 x 14336 bf16 32.7 / 31.6 us; 8192 x 8192 f16 norm with residual 76.1 / 76.0; 1023 x 5003 bf16 norm,
+// element by element, 9.7 / 9.1.)
 template <bool NORM, bool E4M3>
-__device__ __forceinline__ Factor row_factor(const Rows& p, int row, bool active, float sum, float top) {
-    const float r = NORM ? rsqrtf(sum * p.per_col + p.eps) : 1.0f;
-    if (!E4M3) return {r, 1.0f};
-    float most = top * r;
-    if (most < E4M3_MAX * SCALE_MIN) most = E4M3_MAX * SCALE_MIN;   // false for a NaN, which stays
-    if (active && threadIdx.x == 0) p.scales[row] = most / E4M3_MAX;
-    const float inverse = __frcp_rn(most / E4M3_MAX);   // of the scale: the maximum's own would be a subnormal number above 2^126
-    if (NORM && most < SMALL) return {r, inverse};
-    return {r * inverse, 1.0f};
+struct Factor {
+    float lift, high, low;
+    template <int N>
+    __device__ __forceinline__ void operator()(float (&v)[N]) const {
+        if (NORM && E4M3 && lift != 1.0f)   // all threads of a row go one way
+#pragma unroll
+            for (int j = 0; j < N; j++) v[j] *= lift;
+        // Two at a time, the norm into e4m3 is left more of the issue slots (8192 x 8192: 76.4 us, one at a time 77.3); rows that are only
+        // quantised come out of 16-bit pairs and lose more to moves between registers (4096 x 14336: 34.0 us, one at a time 33.3).
+        if constexpr (NORM && E4M3) {
+            const uint64_t h = two(high, high), l = two(low, low);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const uint64_t pair = two(v[j], v[j + 1]), q = fma_two(pair, h, mul_two(pair, l));
+                v[j] = __uint_as_float((uint32_t)q), v[j + 1] = __uint_as_float((uint32_t)(q >> 32));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) v[j] = E4M3 ? fmaf(v[j], high, v[j] * low) : v[j] * high;
+        }
+    }
+};
+constexpr float BELOW = 1.0f - 0x1p-22f;   // more than the hardware's reciprocal is off by
+constexpr float MAX_HIGH = (float)(1.0 / 448.0) * BELOW, MAX_LOW = (float)(1.0 / 448.0 - (double)MAX_HIGH);
+template <bool NORM, bool E4M3>
+__device__ __forceinline__ Factor<NORM, E4M3> row_factor(const Rows& p, int64_t row, bool active, float sum, float top) {
+    float r = 1.0f;
+    if (NORM) {
+        const float square = fmaf(sum, p.per_col_high, sum * p.per_col_low) + p.eps;
+        r = rsqrtf(square);   // the hardware's, two steps off at most; after one of Newton's one
+        if (square >= 0x1p-126f && square <= FLT_MAX) r = fmaf(0.5f * r, fmaf(-square * r, r, 1.0f), r);
+    }
+    if (!E4M3) return {1.0f, r, 0.0f};
+    const float most = top * r;
+    float scale = most < 0x1p-80f ? most / E4M3_MAX : fmaf(most, MAX_HIGH, most * MAX_LOW);   // the nearest to the quotient, which is 1 / 14 of a step or more from any middle
+    if (scale < SCALE_MIN) scale = SCALE_MIN;   // false for a NaN, which stays
+    if (active && threadIdx.x == 0) p.scales[row] = scale;
+    // A norm of rows so small that r / scale could exceed f32 lifts them first, exactly: zeros, first of all, whose r is 1 / sqrt(eps) and whose scale is
+    // 2^-126. Their bytes are zeros, and 0 * inf is none.
+    const float lift = NORM && top < 0x1p-90f ? 0x1p100f : 1.0f;
+    const float divisor = scale * lift;   // 2^-126 to 2^119.2: its reciprocal is a normal number (that of the row's maximum is subnormal above 2^126)
+    float high;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(high) : "f"(divisor));
+    high *= BELOW;
+    float low = fmaf(-high, divisor, 1.0f) * high;
+    if (isinf(divisor)) low = 0.0f;   // a row with an infinity: finite values give 0 * (0 + 0), the infinity NaN
+    if (NORM) {
+        const float product = r * high * BELOW;
+        low = fmaf(r, low, fmaf(r, high, -product));
+        high = product;
+    }
+    return {lift, high, low};
 }
 
 // The largest magnitude in a vector of T; 16-bit values are compared two at a time as they are.
@@ -174,7 +228,8 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
     basalt_k::tc::wait_for_predecessor();
     const int64_t row64 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const bool active = row64 < p.rows;
-    const int row = active ? (int)row64 : 0, vectors = active ? p.cols / W : 0;
+    const int64_t row = active ? row64 : 0;   // times a stride in 64 bits
+    const int vectors = active ? p.cols / W : 0;
     const uint4* x = (const uint4*)((const T*)p.x + row * p.ldx) + threadIdx.x;
     uint4 raw[V];
 #pragma unroll
@@ -223,7 +278,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
         }
     }
     join_row(sum, top);
-    const Factor f = row_factor<NORM, E4M3>(p, row, active, sum, top);
+    const auto f = row_factor<NORM, E4M3>(p, row, active, sum, top);
 #pragma unroll
     for (int v = 0; v < V; v++) {
         if (threadIdx.x + v * blockDim.x >= vectors) continue;
@@ -238,8 +293,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
                 for (int j = 0; j < W; j++) e[j] *= w[j];
             }
         }
-#pragma unroll
-        for (int j = 0; j < W; j++) e[j] = e[j] * f;
+        f(e);
         const int at = (threadIdx.x + v * blockDim.x) * W;
         if constexpr (E4M3) store_e4m3((uint8_t*)p.y + row * p.ldy + at, e);
         else store_vec((T*)p.y + row * p.ldy + at, e);
@@ -252,7 +306,7 @@ constexpr int EACH = 16;
 template <class T, bool NORM, bool RESIDUAL, bool E4M3>
 __global__ void __launch_bounds__(512) rows_by_element(const Rows p) {
     basalt_k::tc::wait_for_predecessor();
-    const int row = blockIdx.x;
+    const int64_t row = blockIdx.x;
     const T* x = (const T*)p.x + row * p.ldx + threadIdx.x;
     const int left = p.cols - threadIdx.x, step = blockDim.x;   // element v of this thread is in the row where v * step < left
     T raw[EACH], more[RESIDUAL ? EACH : 1];
@@ -289,14 +343,15 @@ __global__ void __launch_bounds__(512) rows_by_element(const Rows p) {
         if (E4M3) top = max_nan(top, fabsf(h[v]));
     }
     join_row(sum, top);
-    const Factor f = row_factor<NORM, E4M3>(p, row, true, sum, top);
+    const auto f = row_factor<NORM, E4M3>(p, row, true, sum, top);
+    f(h);
     T* y = (T*)p.y + row * p.ldy + threadIdx.x;
     uint8_t* bytes = (uint8_t*)p.y + row * p.ldy + threadIdx.x;
 #pragma unroll
     for (int v = 0; v < EACH; v++) {
         if (v * step >= left) continue;
-        if constexpr (E4M3) bytes[v * step] = (uint8_t)__nv_cvt_float_to_fp8(h[v] * f, __NV_SATFINITE, __NV_E4M3);
-        else y[v * step] = rounded<T>(h[v] * f);
+        if constexpr (E4M3) bytes[v * step] = one_e4m3(h[v]);
+        else y[v * step] = rounded<T>(h[v]);
     }
 }
 
@@ -305,7 +360,7 @@ __global__ void __launch_bounds__(512) rows_by_element(const Rows p) {
 template <class T, bool NORM, bool E4M3>
 __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
     basalt_k::tc::wait_for_predecessor();
-    const int row = blockIdx.x;
+    const int64_t row = blockIdx.x;
     const T* x = (const T*)p.x + row * p.ldx;
     const T* residual = NORM && p.residual ? (const T*)p.residual + row * p.ldr : nullptr;
     const T* weight = NORM ? (const T*)p.weight : nullptr;
@@ -318,7 +373,7 @@ __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
         top = max_nan(top, fabsf(h));
     }
     join_row(sum, top);
-    const Factor f = row_factor<NORM, E4M3>(p, row, true, sum, top);
+    const auto f = row_factor<NORM, E4M3>(p, row, true, sum, top);
     for (int64_t i = threadIdx.x; i < p.cols; i += blockDim.x) {
         float h = load_one(x + i);
         if (residual) {
@@ -326,8 +381,10 @@ __global__ void __launch_bounds__(512) rows_twice(const Rows p) {
             if (p.total) ((T*)p.total)[row * p.ldt + i] = rounded<T>(h);
         }
         if (weight) h *= load_one(weight + i);
-        if (E4M3) ((uint8_t*)p.y)[row * p.ldy + i] = (uint8_t)__nv_cvt_float_to_fp8(h * f, __NV_SATFINITE, __NV_E4M3);
-        else ((T*)p.y)[row * p.ldy + i] = rounded<T>(h * f);
+        float v[2] = {h, h};
+        f(v);
+        if (E4M3) ((uint8_t*)p.y)[row * p.ldy + i] = one_e4m3(v[0]);
+        else ((T*)p.y)[row * p.ldy + i] = rounded<T>(v[0]);
     }
 }
 
@@ -423,7 +480,8 @@ extern "C" int basalt_k_rms_norm(int type, const void* x, int64_t ldx, const voi
     if (!(eps >= 0.0f)) return basalt_k::record_msg(1, who, "eps must not be negative");
     if (rows == 0) return 0;
     if (const int rc = basalt_k::check_device_pointers(who, {x, residual, total, weight, y, scales})) return rc;
-    const Rows p = {x, residual, weight, total, y, scales, ldx, ldr, ldt, ldy, (int)rows, (int)cols, eps, 1.0f / (float)cols};
+    const float high = (float)(1.0 / (double)cols) * (1.0f - 0x1p-22f);
+    const Rows p = {x, residual, weight, total, y, scales, (int)ldx, (int)ldr, (int)ldt, (int)ldy, (int)rows, (int)cols, eps, high, (float)(1.0 / (double)cols - (double)high)};
     return scales ? launch_type<true, true>(type, p, who, (cudaStream_t)stream) : launch_type<true, false>(type, p, who, (cudaStream_t)stream);
 }
 
@@ -433,6 +491,6 @@ extern "C" int basalt_k_quantize_e4m3(int type, const void* x, int64_t ldx, void
     if (const int rc = check_rows(who, type, rows, cols, {x, rows, cols, ldx, type == BASALT_K_TYPE_F32 ? 4 : 2}, {}, {}, {q, rows, cols, ldq, 1}, scales, nullptr)) return rc;
     if (rows == 0) return 0;
     if (const int rc = basalt_k::check_device_pointers(who, {x, q, scales})) return rc;
-    const Rows p = {x, nullptr, nullptr, nullptr, q, scales, ldx, 0, 0, ldq, (int)rows, (int)cols, 0.0f, 0.0f};
+    const Rows p = {x, nullptr, nullptr, nullptr, q, scales, (int)ldx, 0, 0, (int)ldq, (int)rows, (int)cols, 0.0f, 0.0f, 0.0f};
     return launch_type<false, true>(type, p, who, (cudaStream_t)stream);
 }

@@ -177,7 +177,9 @@ enum { BASALT_K_TYPE_F16 = 0, BASALT_K_TYPE_BF16 = 1, BASALT_K_TYPE_F32 = 2 };
  * in f32, for rows x cols matrices of `type` (F16, BF16, F32) whose rows lie ld* elements apart (cols <= ld < 2^31).
  * residual, total and weight may be NULL (no addition; h not stored; weight 1); total needs residual.
  * scales NULL: y is of `type`.  scales given: y is e4m3 bytes (rows ldy bytes apart) and scales[r] an f32 with
- *   scales[r] = max(max_k |y_k| / 448, 2^-126),   y stored as e4m3(y_k / scales[r]), to the nearest, ties to even.
+ *   scales[r] = max(max_k |y_k| / 448, 2^-126),   y stored as e4m3(y_k / scales[r]), to the nearest, ties to even;
+ * the quotient is an f32 one by the stored scale: exact where f32 holds it, else off by no more than half a step and 2^-30 of it (y is not
+ * rounded before it).
  * The norm goes by h before its rounding to total.  An infinity or a NaN in a row gives what the formulas give; no other
  * row is touched by it.  An output may be an input's own buffer of the same stride and type (total = residual, y = x); any
  * other overlap is refused.  Any alignment and width is right; 16-byte aligned rows of whole 16-byte pieces are read
@@ -186,7 +188,7 @@ int basalt_k_rms_norm(int type, const void *x, int64_t ldx, const void *residual
                       const void *weight, float eps, void *y, int64_t ldy, float *scales, int64_t rows, int64_t cols,
                       void *stream);
 
-/* The quantisation alone: scales[r] = max(max_k |x_k| / 448, 2^-126), q = e4m3(x_k / scales[r]); for the activations between
+/* The quantisation alone: scales[r] = max(max_k |x_k| / 448, 2^-126), the nearest f32, and q = e4m3(x_k / scales[r]) as above; for the activations between
  * two products, and for weights (rows = output channels).  Arguments as above. */
 int basalt_k_quantize_e4m3(int type, const void *x, int64_t ldx, void *q, int64_t ldq, float *scales, int64_t rows,
                            int64_t cols, void *stream);

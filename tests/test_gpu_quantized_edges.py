@@ -56,3 +56,62 @@ def test_norm_to_e4m3_of_the_largest_weights(gpu, cols):
     _, want = exact_norm(x, None, w, 1e-6)
     assert want.abs().amax(1).min() > 2.0 ** 126
     check_e4m3(down(dy, y), down(ds, s), want, (cols / 2 + 10) * U)
+
+
+def e4m3_of_the_quotient(y, s):
+    """y / s in f32, as the CPU divides, then e4m3 to the nearest, ties to even."""
+    return (y.float() / s[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+def rows_of_ties(cols, t, exponent):
+    """Rows whose largest magnitude is 448 * 2^exponent, so that the scale is 2^exponent, and whose other values are e4m3 numbers and the points
+    half-way between two of them, of both signs: odd multiples of half a step, the subnormals' among them, and zeros."""
+    e4m3 = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    points = torch.cat([e4m3, (e4m3[1:] + e4m3[:-1]) / 2])
+    points = torch.cat([points, -points])
+    x = points[torch.randint(0, len(points), (3, cols), generator=gen(cols))]
+    x[:, cols - 1] = 448.0
+    x = (x * 2.0 ** exponent).to(T[t])
+    assert torch.equal((x.double() * 2.0 ** -exponent * 1024).frac(), torch.zeros(3, cols, dtype=torch.float64))   # nothing was rounded
+    return x
+
+
+@pytest.mark.parametrize("t,exponent", [("f16", 0), ("f16", 6), ("bf16", 0), ("bf16", 119), ("bf16", -100), ("f32", 0), ("f32", -126), ("f32", -91), ("f32", -90), ("f32", 100)])
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_quantize_ties_go_to_even(gpu, cols, t, exponent):
+    x = rows_of_ties(cols, t, exponent)
+    q, s = quantized(gpu, x, t)
+    assert (s == 2.0 ** exponent).all()
+    assert torch.equal(q, e4m3_of_the_quotient(x, s))
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("cols", WIDTHS)
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -9, 700.0])
+def test_quantize_is_the_quotient_by_the_stored_scale(gpu, cols, t, scale):
+    """The scale is the f32 quotient max / 448, the bytes are those of the f32 quotient x / scale. (A quotient that f32 holds is met exactly and
+    any other within half a step and 2^-45 of it, so that a byte could differ from these only where a division comes as near as that
+    to the middle of two f32 numbers; none of 24 bits by 24 does outside subnormals.) 16-bit rows meet ties often."""
+    x = rows(gen(cols), 40 if cols < 9000 else 5, cols, T[t], 0, scale)
+    q, s = quantized(gpu, x, t)
+    assert torch.equal(s, x.float().abs().amax(1) / torch.full((x.shape[0],), 448.0))
+    assert torch.equal(q, e4m3_of_the_quotient(x, s))
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("cols", WIDTHS)
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_to_e4m3_ties_go_to_even(gpu, cols, t, residual):
+    """h = +-1 and eps = 0: the mean of squares and its root are exactly one, y is the weight with h's sign, and ties are ties."""
+    w = rows_of_ties(cols, t, 0)[0]
+    h = torch.where(torch.rand(3, cols, generator=gen(cols)) < 0.5, -1.0, 1.0).to(T[t])
+    r = torch.randint(-4, 5, (3, cols), generator=gen(cols + 1)).to(T[t])
+    x = h - r if residual else h
+    y, s = torch.full((3, cols), 0x55, dtype=torch.uint8), torch.full((3,), 5.0)
+    dy, ds = up(gpu, y), up(gpu, s)
+    total = up(gpu, torch.zeros_like(x)) if residual else None
+    kernels.rms_norm(up(gpu, x), dy, 3, cols, t, weight=up(gpu, w), eps=0.0, residual=up(gpu, r) if residual else None, total=total, scales=ds)
+    gpu.synchronize()
+    q, s = down(dy, y), down(ds, s)
+    assert (s == 1.0).all()
+    assert torch.equal(q, e4m3_of_the_quotient(h.float() * w.float(), s))
