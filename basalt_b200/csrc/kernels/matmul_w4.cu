@@ -44,6 +44,13 @@ __device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, int
 // Arrives on the barrier when every copy that this thread has begun is done.
 __device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory"); }
 
+// For every reader of a ring's place, before the warp hands it back: orders what the thread has read there before the bulk loads that fill it again. They write
+// through the async proxy, which an arrival on a barrier alone does not order against plain reads: without this, reads that queued behind the copies' cache
+// misses saw the next slab (14720 -> 14931 in groups of 32, bf16, from cold memory, with a warp that only carries scales: one launch in four missed 32 k of X
+// in the rows of a warp on that warp's scheduler; without such a warp one in a hundred).
+// It costs 0.5 us of 20.5 for 17 rows through 8192 x 8192, nothing that shows for one row.
+__device__ __forceinline__ void reads_done() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // A slab's scales and zero points in shared memory: of each of the tile's 128 rows the groups that 256 k touch, at most 8 / FLUSH where
 // FLUSH * 32 k certainly share a group. They travel with the slab's weights. (A load by each thread that wants a scale touches 32
 // rows, so 32 lines of the cache, in an instruction: with those, one row through 8192 x 8192 in groups of 32 took 34 us.)
@@ -340,6 +347,7 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
                         for (int j = 0; j < 2; j++) total[r >> 1][nt][2 * (r & 1) + j] += b * acc[r >> 1][nt][2 * (r & 1) + j];
                 }
             }
+            reads_done();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
             if (++s == STAGES) s = 0, ph ^= 1;
@@ -603,6 +611,7 @@ __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_c
                     unpack_scaled<T>(w.x, z2[h], s2[h], out + 16 * h), unpack_scaled<T>(w.y, z2[h], s2[h], out + 16 * h + 4);
                     unpack_scaled<T>(w.z, z2[h], s2[h], out + 16 * h + 8), unpack_scaled<T>(w.w, z2[h], s2[h], out + 16 * h + 12);
                 }
+                reads_done();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&raw_empty[rs]));
                 if (++rs == p.raws) rs = 0, rph ^= 1;

@@ -115,3 +115,32 @@ def test_norm_to_e4m3_ties_go_to_even(gpu, cols, t, residual):
     q, s = down(dy, y), down(ds, s)
     assert (s == 1.0).all()
     assert torch.equal(q, e4m3_of_the_quotient(h.float() * w.float(), s))
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("K", [14720, 14848])   # groups of 32, 64 and 128 in whole aligned pieces in the second only
+@pytest.mark.parametrize("group", [32, 64, 96, 128])
+def test_matmul_w4_in_every_form_from_cold_memory(gpu, group, K, zeros, t):
+    """Every launch is compared, the caches overwritten before it: the scales of a slab take longest to come then, and have to be waited for. M
+    goes through tiles of 8 and 16 rows and through narrow, middling and wide tiles of the tcgen05 kernel."""
+    N, dev = 14931, "cuda"
+    g = torch.Generator(device=dev)
+    g.manual_seed(group + K)
+    groups = -(-K // group)
+    q = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8, device=dev)
+    s = (2.0 ** torch.randint(-2, 2, (N, groups), generator=g, device=dev).float()).to(T[t])
+    z = torch.randint(0, 16, (N, groups), generator=g, dtype=torch.uint8, device=dev) if zeros else None
+    at = torch.arange(K, device=dev) // group
+    w = (q.float() - (8.0 if z is None else z.float()[:, at])) * s.float()[:, at]
+    packed = q[:, 0::2] | (q[:, 1::2] << 4)
+    caches = torch.empty(256 << 20, dtype=torch.uint8, device=dev)
+    stream = torch.cuda.current_stream().cuda_stream
+    for M in (1, 9, 64, 150, 300):
+        x = torch.randint(-2, 3, (M, K), generator=g, device=dev).to(T[t])
+        want = (x.float() @ w.T).to(T[t])   # quarters below 2^20: exact in 32 bits in any order
+        c = torch.empty(M, N, dtype=T[t], device=dev)
+        for i in range(60):
+            caches.fill_(i)
+            kernels.matmul_w4(x.data_ptr(), packed.data_ptr(), s.data_ptr(), c.data_ptr(), M, N, K, group, t, zeros=None if z is None else z.data_ptr(), stream=stream)
+            assert torch.equal(c, want), (M, i, int((c != want).sum()))
