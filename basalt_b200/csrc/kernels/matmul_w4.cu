@@ -47,7 +47,7 @@ __device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.a
 // For every reader of a ring's place, before the warp hands it back: orders what the thread has read there before the bulk loads that fill it again. They write
 // through the async proxy, which an arrival on a barrier alone does not order against plain reads: without this, reads that queued behind the copies' cache
 // misses saw the next slab (14720 -> 14931 in groups of 32, bf16, from cold memory, with a warp that only carries scales: one launch in four missed 32 k of X
-// in the rows of a warp on that warp's scheduler; without such a warp one in a hundred).
+// in the rows of a warp on that warp's scheduler).
 // It costs 0.5 us of 20.5 for 17 rows through 8192 x 8192, nothing that shows for one row.
 __device__ __forceinline__ void reads_done() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -793,11 +793,7 @@ int launch_tall(const Args& p, const TallPlan& plan) {
 // 13.7 / 10.0; 17 rows, 8192 -> 8192: 23.7 / 21.0.) Under 128 rows of weights most of the tcgen05 kernel's lanes would idle.
 template <class T, int FLUSH, bool ZEROS>
 int launch_rows(const Args& p) {
-    // Tiles of eight rows only where a slab has at most four groups: with eight, four stages deep, copies of scales were seen to be read before they
-    // were there (one row, 14720 -> 14931 in groups of 32, from cold memory: one row of the weights in a hundred off by a slab's scales); tiles of 16,
-    // three deep, gave the same bits in 25,000 such runs.
-    if constexpr (FLUSH > 1)
-        if (p.M <= 8) return launch_few<T, 1, FLUSH, ZEROS>(p);
+    if (p.M <= 8) return launch_few<T, 1, FLUSH, ZEROS>(p);
     if (p.M > 16 && p.N >= ROWS) {
         const int slabs = (p.K - 1) / few::SLAB_K + 1;
         const int64_t tiles = (int64_t)((p.M - 1) / 16 + 1) * ((p.N - 1) / ROWS + 1);
