@@ -19,7 +19,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libbasalt_b200.so")
 CLI = os.path.join(HERE, "basalt-b200")
-PYTHON_BINDING = os.path.join(HERE, "_klaunch.so")
+PYTHON_BINDING = os.path.join(HERE, "_klaunch" + sysconfig.get_config_var("EXT_SUFFIX"))   # each interpreter has its own
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 
 CXX_SOURCES = ["bir.cpp", "passes.cpp", "emit.cpp", "emit_mma.cpp", "regbudget.cpp", "frontend_c.cpp", "frontend_triton.cpp", "capi.cpp", "runtime.cpp"]
@@ -71,11 +71,15 @@ def _build_shims(force: bool, run) -> None:
 
 
 def _build_python_binding(force: bool, run) -> None:
-    """_klaunch.so: the CPython binding of the launch-bound kernels, linked against the library beside it."""
-    src = os.path.join(CSRC, "python_binding.cpp")
-    if force or _stale(PYTHON_BINDING, [src, LIB, os.path.abspath(__file__)]):
-        run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{sysconfig.get_paths()['include']}", "-o", PYTHON_BINDING, src, f"-L{HERE}",
-             "-lbasalt_b200", "-Wl,-rpath,$ORIGIN"])
+    """_klaunch: the CPython binding of the launch-bound kernels, linked against the library beside it. An interpreter without its
+    headers goes without: basalt_b200.kernels then says so where one of its functions is called."""
+    src, include = os.path.join(CSRC, "python_binding.cpp"), sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        print(f"{include}/Python.h not found: the Python binding of the quantised layer's kernels is not built", file=sys.stderr)
+        return
+    header = os.path.join(CSRC, "../../include/basalt_b200_kernels.h")
+    if force or _stale(PYTHON_BINDING, [src, header, LIB, os.path.abspath(__file__)]):
+        run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{include}", "-o", PYTHON_BINDING, src, f"-L{HERE}", "-lbasalt_b200", "-Wl,-rpath,$ORIGIN"])
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -4,9 +4,13 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import _klaunch
 from ._lib import lib
 from .runtime import DeviceBuffer
+
+try:
+    from . import _klaunch
+except ImportError as e:
+    _klaunch, _klaunch_missing = None, e
 
 
 class KernelError(Exception):
@@ -94,33 +98,41 @@ def sgemm_f32_variant(A, B, Cm, M: int, N: int, K: int, no_tail_split: bool = Fa
 TYPES = {"f16": 0, "bf16": 1, "f32": 2}
 
 
+def _fast():
+    """The CPython binding: the four functions below go through it instead of ctypes, whose conversion of their arguments would take
+    longer than the launch."""
+    if _klaunch is None:
+        raise ImportError(f"basalt_b200._klaunch is missing ({_klaunch_missing}): build it for this interpreter with `python -m basalt_b200.build` (needs Python.h); "
+                          "the C entry points and the other functions of this module do without it")
+    return _klaunch
+
+
 def _type(name: str) -> int:
     if name not in TYPES:
         raise KernelError(f"unknown type {name!r}: one of {', '.join(TYPES)}")
     return TYPES[name]
 
 
-# The four below go through a CPython binding instead of ctypes, whose conversion of their arguments would take longer than the launch.
-# Pointers are ints, DeviceBuffers or None.
+# Pointers of the four below are ints, DeviceBuffers or None.
 
 def rms_norm(x, y, rows: int, cols: int, dtype: str, weight=None, eps: float = 1e-6, residual=None, total=None, scales=None, ldx=None, ldy=None,
              ldr=None, ldt=None, stream=None):
     """y = (x + residual) * weight / rms over rows of `dtype`; `total` receives x + residual. With `scales` (f32, one a row) y is
     e4m3, y / scales[row]. Strides are in elements and default to cols."""
-    _check(_klaunch.rms_norm(_type(dtype), x, ldx, residual, ldr, total, ldt, weight, eps, y, ldy, scales, rows, cols, stream))
+    _check(_fast().rms_norm(_type(dtype), x, ldx, residual, ldr, total, ldt, weight, eps, y, ldy, scales, rows, cols, stream))
 
 
 def quantize_e4m3(x, q, scales, rows: int, cols: int, dtype: str, ldx=None, ldq=None, stream=None):
     """q = e4m3(x / scales[row]) with scales[row] = max|x| / 448, row by row."""
-    _check(_klaunch.quantize_e4m3(_type(dtype), x, ldx, q, ldq, scales, rows, cols, stream))
+    _check(_fast().quantize_e4m3(_type(dtype), x, ldx, q, ldq, scales, rows, cols, stream))
 
 
 def matmul_e4m3(A, a_scales, B, b_scales, Cm, M: int, N: int, K: int, out: str = "f16", lda=None, ldb=None, ldc=None, status=None, stream=None):
     """C = (A * B^T) * a_scales[m] * b_scales[n] of e4m3 A [M x K] and B [N x K]; C of type `out`. Row strides default to K, K and N."""
-    _check(_klaunch.matmul_e4m3(A, lda, a_scales, B, ldb, b_scales, _type(out), Cm, ldc, M, N, K, status, stream))
+    _check(_fast().matmul_e4m3(A, lda, a_scales, B, ldb, b_scales, _type(out), Cm, ldc, M, N, K, status, stream))
 
 
 def matmul_w4(X, W, scales, Cm, M: int, N: int, K: int, group: int, dtype: str = "f16", zeros=None, ldx=None, ldw=None, ldc=None, status=None, stream=None):
     """C = X * ((q - zeros) * scales)^T with 4-bit q packed two to a byte in W [N x K/2], scales and zeros per `group` of k.
     ldx and ldc count elements, ldw bytes; they default to K, N and the packed row."""
-    _check(_klaunch.matmul_w4(_type(dtype), X, ldx, W, ldw, scales, zeros, group, Cm, ldc, M, N, K, status, stream))
+    _check(_fast().matmul_w4(_type(dtype), X, ldx, W, ldw, scales, zeros, group, Cm, ldc, M, N, K, status, stream))
