@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from basalt_b200 import kernels
-from test_gpu_quantized import T, U, check_e4m3, down, exact_norm, gen, rows, up
+from test_gpu_quantized import T, U, check_e4m3, down, e4m3_rows, exact_norm, gen, rows, run_e4m3, up
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,17 @@ def test_matmul_w4_in_every_form_from_cold_memory(gpu, group, K, zeros, t):
             caches.fill_(i)
             kernels.matmul_w4(x.data_ptr(), packed.data_ptr(), s.data_ptr(), c.data_ptr(), M, N, K, group, t, zeros=None if z is None else z.data_ptr(), stream=stream)
             assert torch.equal(c, want), (M, i, int((c != want).sum()))
+
+
+@pytest.mark.parametrize("ldc_pad", [0, 4, 3])   # C's rows are whole 16-byte pieces, with a gap or without one, or not
+@pytest.mark.parametrize("shape", [(1000, 2600, 16300), (1030, 2100, 8200), (600, 4100, 24600), (150, 700, 20000), (5, 68, 16400)])
+def test_matmul_e4m3_parts_are_added_to_f32(gpu, shape, ldc_pad):
+    """A K beyond 8192 in two, three and four parts, the later ones added to what C holds: on pairs of CTAs (the first three shapes) in whole pieces and element by
+    element, and in narrower tiles. Sums of small integers below 2^24 are exact whatever their order."""
+    M, N, K = shape
+    g = gen(M + K)
+    a, b = torch.randint(-3, 4, (M, K), generator=g).float(), torch.randint(-2, 3, (N, K), generator=g).float()
+    sa, sb = 2.0 ** torch.randint(-3, 3, (M,), generator=g).float(), 2.0 ** torch.randint(-2, 3, (N,), generator=g).float()
+    want = (a @ b.T) * sa[:, None] * sb
+    got = run_e4m3(gpu, e4m3_rows(a, 5), sa, e4m3_rows(b, 0), sb, K, "f32", ldc_pad)
+    assert torch.equal(got, want), int((got != want).sum())
