@@ -24,11 +24,14 @@ struct Span {
     int64_t rows, cols, ld;
     int size;
 };
-// Whether the address ranges of two matrices meet.
+// Whether two matrices have bytes in common. Two of one stride whose columns lie beside one another (the halves of a wider buffer's rows) have none.
 inline bool overlap(const Span& a, const Span& b) {
     if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
     const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
-    return a0 < b0 + (uintptr_t)(((b.rows - 1) * b.ld + b.cols) * b.size) && b0 < a0 + (uintptr_t)(((a.rows - 1) * a.ld + a.cols) * a.size);
+    if (a0 >= b0 + (uintptr_t)(((b.rows - 1) * b.ld + b.cols) * b.size) || b0 >= a0 + (uintptr_t)(((a.rows - 1) * a.ld + a.cols) * a.size)) return false;
+    if (a.ld * a.size != b.ld * b.size || a.cols > a.ld || b.cols > b.ld) return true;
+    const int64_t stride = a.ld * a.size, step = (int64_t)(b0 - a0) % stride, at = step < 0 ? step + stride : step;   // of b's first column, from a's
+    return at < a.cols * a.size || at + b.cols * b.size > stride;
 }
 
 // Lets KERNEL have `bytes` of dynamic shared memory on the current device; asked of the runtime once a kernel and device.

@@ -168,7 +168,8 @@ int basalt_k_fill(int kind, uint64_t seed, uint64_t start, int64_t n, void *out,
 
 /* ---- A quantised linear layer around the matmul: norm, row quantisation, e4m3 and 4-bit products ----
  *
- * Row strides lie below 2^31; M, N and K of the products do not exceed 2^30.  C overlaps no input.
+ * Row strides lie below 2^31; M, N and K of the products do not exceed 2^30.  C overlaps no input; matrices of one row stride (in bytes) may
+ * lie beside one another in a wider buffer's rows.
  * The reference has no counterpart to these four. Element types of matrices and vectors: */
 enum { BASALT_K_TYPE_F16 = 0, BASALT_K_TYPE_BF16 = 1, BASALT_K_TYPE_F32 = 2 };
 

@@ -1,6 +1,9 @@
 """Calls of the quantised layer's operators at the ends of their ranges: the largest rows, exact ties, weights from cold
 memory, long sums, matrices that share a buffer."""
-import numpy as np
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -8,6 +11,7 @@ from basalt_b200 import kernels
 from test_gpu_quantized import T, U, check_e4m3, down, e4m3_rows, exact_norm, gen, rows, run_e4m3, up
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 # widths of every path through the row kernels: whole vectors in registers, element by element, and read twice
 WIDTHS = [64, 77, 4096, 9001, 40000]
@@ -158,3 +162,58 @@ def test_matmul_e4m3_parts_are_added_to_f32(gpu, shape, ldc_pad):
     want = (a @ b.T) * sa[:, None] * sb
     got = run_e4m3(gpu, e4m3_rows(a, 5), sa, e4m3_rows(b, 0), sb, K, "f32", ldc_pad)
     assert torch.equal(got, want), int((got != want).sum())
+
+
+@pytest.mark.parametrize("cols", [64, 77, 4096, 9001])
+def test_norm_beside_its_input_in_one_buffer(gpu, cols):
+    g = gen(cols)
+    both = torch.cat([rows(g, 5, cols, torch.bfloat16), torch.full((5, cols), 3.0, dtype=torch.bfloat16)], 1)
+    w = rows(g, 1, cols, torch.bfloat16)
+    db, dw, dx, dy = up(gpu, both), up(gpu, w), up(gpu, both[:, :cols].contiguous()), up(gpu, both[:, cols:].contiguous())
+    kernels.rms_norm(db, db.device_ptr() + 2 * cols, 5, cols, "bf16", weight=dw, ldx=2 * cols, ldy=2 * cols)
+    kernels.rms_norm(dx, dy, 5, cols, "bf16", weight=dw)
+    gpu.synchronize()
+    got = down(db, both)
+    assert torch.equal(got[:, :cols], both[:, :cols]) and torch.equal(got[:, cols:], down(dy, torch.empty(5, cols, dtype=torch.bfloat16)))
+
+
+@pytest.mark.parametrize("M", [3, 20, 300])
+def test_products_beside_their_input_in_one_buffer(gpu, M):
+    K = N = 256
+    g = gen(M)
+    x, q, s = torch.randint(-2, 3, (M, K), generator=g).half(), torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8), torch.ones(N, K // 32, dtype=torch.float16)
+    both = torch.cat([x, torch.full((M, N), 7.0, dtype=torch.float16)], 1)
+    db = up(gpu, both)
+    kernels.matmul_w4(db, up(gpu, q[:, 0::2] | (q[:, 1::2] << 4)), up(gpu, s), db.device_ptr() + 2 * K, M, N, K, 32, "f16", ldx=2 * K, ldc=2 * K)
+    got = down(db, both)
+    assert torch.equal(got[:, :K], x) and torch.equal(got[:, K:], (x.float() @ (q.float() - 8).T).half())
+    a, b = torch.randint(-3, 4, (M, K), generator=g).float(), torch.randint(-2, 3, (N // 2, K), generator=g).float()
+    both = torch.cat([e4m3_rows(a, 0), torch.full((M, N), 1, dtype=torch.uint8)], 1)   # 256 bytes of A, 128 f16 of C
+    db = up(gpu, both)
+    kernels.matmul_e4m3(db, up(gpu, torch.ones(M)), up(gpu, e4m3_rows(b, 0)), up(gpu, torch.ones(N // 2)), db.device_ptr() + K, M, N // 2, K, "f16", lda=2 * K, ldc=K)
+    got = down(db, both)
+    assert torch.equal(got[:, :K], both[:, :K]) and torch.equal(got[:, K:].contiguous().view(torch.float16), (a @ b.T).half())
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from basalt_b200 import kernels
+x, w, q, s = torch.randn(4, 512, device="cuda").half(), torch.ones(512, device="cuda").half(), torch.empty(4, 512, dtype=torch.uint8, device="cuda"), torch.empty(4, device="cuda")
+b, bs, c = torch.zeros(256, 512, dtype=torch.uint8, device="cuda"), torch.ones(256, device="cuda"), torch.ones(4, 256, device="cuda").half()
+w4, w4s, c4 = torch.full((256, 256), 0x99, dtype=torch.uint8, device="cuda"), torch.ones(256, 4, device="cuda").half(), torch.zeros(4, 256, device="cuda").half()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    st = torch.cuda.current_stream().cuda_stream
+    kernels.rms_norm(x.data_ptr(), q.data_ptr(), 4, 512, "f16", weight=w.data_ptr(), scales=s.data_ptr(), stream=st)
+    kernels.matmul_e4m3(q.data_ptr(), s.data_ptr(), b.data_ptr(), bs.data_ptr(), c.data_ptr(), 4, 256, 512, "f16", stream=st)
+    kernels.matmul_w4(x.data_ptr(), w4.data_ptr(), w4s.data_ptr(), c4.data_ptr(), 4, 256, 512, 128, "f16", stream=st)
+graph.replay()
+torch.cuda.synchronize()
+assert (c == 0).all() and (s > 0).all() and torch.allclose(c4.float(), x.float().sum(1, keepdim=True).expand(4, 256), rtol=2**-10, atol=2**-10)
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(gpu):
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
