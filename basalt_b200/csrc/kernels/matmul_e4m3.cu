@@ -65,9 +65,11 @@ __device__ __forceinline__ void store_sum(T* c, float v, int add) {
     store_as(c, v);
 }
 
+// The scales are no __restrict__ pointers here and below: the kernel before, which may still run when this one begins, writes them, and a pointer that
+// promises memory nobody writes could be read before the wait for it.
 template <class T, int TN>
 __global__ void __launch_bounds__(THREADS) matmul_e4m3_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
-                                                              const float* __restrict__ a_scales, const float* __restrict__ b_scales, T* __restrict__ C,
+                                                              const float* a_scales, const float* b_scales, T* __restrict__ C,
                                                               int64_t ldc, int M, int N, int K, int shift, int add, int32_t* status) {
     constexpr int STAGES = stages_of<TN>(), A_BYTES = TN * BK, STAGE_BYTES = B_BYTES + A_BYTES;
     constexpr uint32_t TMEM_COLS = TN < 32 ? 32 : TN;
@@ -209,8 +211,8 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* m,
 // VECTORS: C's rows are whole 16-byte pieces from an aligned start.
 template <class T, bool VECTORS>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
-    matmul_e4m3_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const float* __restrict__ a_scales,
-                     const float* __restrict__ b_scales, T* __restrict__ C, int64_t ldc, int M, int N, int K, int add, int32_t* status) {
+    matmul_e4m3_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const float* a_scales,
+                     const float* b_scales, T* __restrict__ C, int64_t ldc, int M, int N, int K, int add, int32_t* status) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tfull_bar[2], tempty_bar[2];
     __shared__ uint32_t tmem_slot;

@@ -195,6 +195,30 @@ def test_products_beside_their_input_in_one_buffer(gpu, M):
     assert torch.equal(got[:, :K], both[:, :K]) and torch.equal(got[:, K:].contiguous().view(torch.float16), (a @ b.T).half())
 
 
+@pytest.mark.parametrize("M", [1, 40, 600])
+def test_the_scales_of_the_norm_before_reach_the_product(gpu, M):
+    """The product's kernel begins while the norm still runs; what it reads of the scales has to be this norm's, not the one's before."""
+    K, N, n = 4096, 520, 40
+    g = gen(M)
+    b = e4m3_rows((torch.randn(N, K, generator=g) * 40).clamp(-448, 448), 0)
+    db, dbs, dq, dqs = up(gpu, b), up(gpu, torch.full((N,), 0.01)), up(gpu, torch.zeros(M, K, dtype=torch.uint8)), up(gpu, torch.zeros(M))
+    xs = [up(gpu, torch.randn(M, K, generator=g).half() * 1.5 ** (i % 7)) for i in range(n)]
+    out = []
+    for wait in (True, False):
+        cs = [up(gpu, torch.zeros(M, N)) for _ in range(n)]
+        for x, c in zip(xs, cs):
+            kernels.quantize_e4m3(x, dq, dqs, M, K, "f16")
+            if wait:
+                gpu.synchronize()
+            kernels.matmul_e4m3(dq, dqs, db, dbs, c, M, N, K, "f32")
+            if wait:
+                gpu.synchronize()
+        gpu.synchronize()
+        out.append([down(c, torch.empty(M, N)) for c in cs])
+    for apart, together in zip(*out):
+        assert torch.equal(apart, together)
+
+
 FIRST_CALL_CAPTURED = """
 import torch
 from basalt_b200 import kernels
