@@ -14,7 +14,7 @@
 // 256 columns at most, with them; no CTA that waits for its cluster can be kept from starting by another's.)
 // Ragged edges are the tensor maps' business: what lies outside a matrix is read as zero.
 // What bounds it: for one row the weights, 14.2 us for 8192 x 8192 (4.7 TB/s; a plain stream of as many bytes takes 11.4 to 12.3, the rest is the
-// way of the first and the last slab); for many rows see the pairs of CTAs below, 8192^3 in 362 to 372 us in a burst (3.0 PFLOP/s) and 413 to 441 at the 1.25 GHz
+// way of the first and the last slab); for many rows see the pairs of CTAs below, 8192^3 in 374 to 382 us in a burst (2.9 PFLOP/s) and 419 to 445 at the 1.2 GHz
 // that the power cap leaves.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -500,7 +500,8 @@ extern "C" int basalt_k_matmul_e4m3(const void* A, int64_t lda, const float* a_s
     if (c_type == BASALT_K_TYPE_F16) return launch_type<__half>(p);
     if (c_type == BASALT_K_TYPE_BF16) return launch_type<__nv_bfloat16>(p);
     // The tensor cores' f32 sums are truncated, term by term, which costs some 9e-11 of the result for each k: 1.4e-6 at 16,384. An f32 result
-    // shows it, so K goes in equal parts of at most 8192, each rounded and added to C in turn.
+    // shows it, so K goes in equal parts of at most 8192, each rounded and added to C in turn. (What that and the wider C cost, f32 / f16: 2048 rows,
+    // 16384 -> 4096, 172 / 92 us; one row 19.4 / 14.8.)
     const int parts = (K - 1) / PART_K + 1, part = ((K - 1) / parts / BK + 1) * BK;
     for (int k = 0; k < K; k += part) {
         Args q = p;

@@ -196,9 +196,10 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 // 32-bit word of packed weights (eight k) and one 16-byte load of X (eight k) feed two instructions without a shuffle
 // between threads. (tcgen05.mma would save the products, which are not what bounds this: its instructions are 128 rows high, and
 // a group's sum would have to leave tensor memory before its scale.)
-// What bounds it: logic operations, half a warp a clock. Unpacking eight weights takes five of them (seven in bf16), a tile's
-// share of ordering X one more, 7 us of the 11.4 that one row through 8192 x 8192 takes (2.9 TB/s of packed weights; a plain stream of as many bytes
-// takes 6.5). 16 rows, 4096 -> 14336 in groups of 64 with zero points, bf16: 18.2 us.
+// What bounds it: no unit by itself. One row through 8192 x 8192 takes 11.8 to 12.2 us (2.9 TB/s of packed weights; a plain stream of as many bytes takes
+// 6.5) with the memory 28 % busy, the issue slots 44 % and the logic unit, which unpacks, 36 %: a warp has one slab's chain of barrier, scales, unpacking,
+// product and scaled sum in flight, and shares of K in powers of two leave places empty (256 CTAs on 148 SMs that hold two each).
+// 16 rows, 4096 -> 14336 in groups of 64 with zero points, bf16: 18.9 us; one row in groups of 32: 14.3, bf16 with zero points 17.6.
 namespace few {
 constexpr int SLAB_K = 256, W_BYTES = ROWS * SLAB_K / 2, CONSUMERS = 8, THREADS = 32 * (CONSUMERS + 1), X_BOX_K = 32;
 
@@ -395,9 +396,9 @@ __global__ void __launch_bounds__(THREADS, 2) matmul_w4_kernel(const __grid_cons
 // a step a weight, of random sign, beside the one of C: the error of C grows by less than the root of two.
 // (Through shared memory, written once and read by every MMA, the operand made that memory the bound: 2048 rows, 11008 -> 4096, 149 us
 // where this took 122.) Persistent where there are more tiles than SMs; a cluster shares a tile's K where there are fewer.
-// What bounds it: for wide tiles the tensor cores at the clock the power cap leaves (2048 rows, 11008 -> 4096: 1.3 PFLOP/s at 138 to 141 us in a burst,
-// 1.18 at 156 in a longer run); for narrow ones the way of a slab from barrier to barrier, some 0.27 us of 64 k (64 rows,
-// 8192 x 8192: 22.4 us, where the weights alone would take 5.3).
+// What bounds it: for wide tiles the tensor cores at the clock the power cap leaves (2048 rows, 11008 -> 4096: 1.3 PFLOP/s at 141 to 142 us in a burst,
+// 1.12 at 165 in a longer run); for narrow ones the way of a slab from barrier to barrier, some 0.28 us of 64 k (64 rows,
+// 8192 x 8192: 22.9 us, where the weights alone would take 5.3).
 namespace tall {
 constexpr int SLAB_K = 256, TILE_K = 64, PACKED_BYTES = ROWS * SLAB_K / 2, MAX_STAGES = 8, MAX_RAW = 4, MAX_M = 256;
 constexpr int WARP_X = 0, WARP_MMA = 1, WARP_RAW = 2, TEAMS = SLAB_K / TILE_K, TEAM = 4, FIRST_UNPACKER = 4, EPILOGUE = 4;
@@ -423,8 +424,8 @@ struct Shape {
 };
 
 // HALVES: 64-k tiles in a stage. Two, wherever three such stages fit (tiles of up to 240 columns): the tensor cores run dry while the
-// issuing thread waits for a stage and its barrier's answer, some 250 clocks (64 rows, 8192 x 8192: 24.5 us with one, 22.4 with two; 2048
-// rows, 11008 -> 4096, under the power cap: 170 and 156).
+// issuing thread waits for a stage and its barrier's answer, some 250 clocks (before reads_done() was needed, 64 rows, 8192 x 8192: 24.5 us with one, 22.4 with
+// two; 2048 rows, 11008 -> 4096, under the power cap: 170 and 156).
 template <class T, int FLUSH, bool ZEROS, int HALVES>
 __global__ void __launch_bounds__(TALL_THREADS, 1) matmul_w4_tall(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                   const T* __restrict__ scales, const uint8_t* __restrict__ zeros, T* __restrict__ C,
@@ -742,7 +743,7 @@ int launch_few(const Args& p) {
 
 // The width of a tile of the tcgen05 kernel and the CTAs that share its K (one CTA fits an SM): of the few counts of tiles over M that come near
 // 256 columns each, the one that costs least. A slab costs what its products do, two clocks a column and 64 k, and not less than
-// its unpacking, about 112 columns' worth. (128 rows through 8192 x 8192: tiles of 128 with K shared 24.5 us, of 64 without 37.)
+// its unpacking, about 112 columns' worth. (128 rows through 8192 x 8192: tiles of 128 with K shared 25.4 us, of 64 without some 37.)
 struct TallPlan {
     int width, tiles, shift;
     double time;   // us
@@ -789,8 +790,8 @@ int launch_tall(const Args& p, const TallPlan& plan) {
 }
 
 // Up to 16 rows go through the kernel for few rows. More do so in tiles of 16, where that is the shorter way: 2.5 us and 1.6 a slab and
-// round of CTAs against the estimate above. (Tiles of 16 / tcgen05, measured: 48 rows, 4096 -> 1024: 6.9 / 8.9 us; 64 rows, 4096 -> 4096:
-// 13.7 / 10.0; 17 rows, 8192 -> 8192: 23.7 / 21.0.) Under 128 rows of weights most of the tcgen05 kernel's lanes would idle.
+// round of CTAs against the estimate above. (Tiles of 16 / tcgen05, measured: 48 rows, 4096 -> 1024: 7.2 / 8.9 us; 64 rows, 4096 -> 4096:
+// 13.9 / 10.5; 17 rows, 8192 -> 8192: 24.4 / 21.1; 64 rows, 2048 -> 2048: 7.1 / 7.5.) Under 128 rows of weights most of the tcgen05 kernel's lanes would idle.
 template <class T, int FLUSH, bool ZEROS>
 int launch_rows(const Args& p) {
     if (p.M <= 8) return launch_few<T, 1, FLUSH, ZEROS>(p);

@@ -10,8 +10,8 @@
 // row, one exchange between the row's threads joins both numbers, and the row is written from registers:
 // every input is read once and every output written once.
 //
-// What bounds it: memory. 8192 x 8192 in f16 with a residual to e4m3: 470 MB in 72.0 us, 6.5 TB/s, what a plain copy reaches; 4096 x 14336 bf16 to
-// e4m3: 176 MB in 29.7 us, 5.9 TB/s. One row of 4096 takes 2.1 us, a launch's time.
+// What bounds it: memory. 8192 x 8192 in f16 with a residual to e4m3: 470 MB in 72.2 us, 6.5 TB/s, what a plain copy reaches; 4096 x 14336 bf16 to
+// e4m3: 176 MB in 30.8 us, 5.7 TB/s, with 69 % of the issue slots taken. One row of 4096 takes 2.1 us, a launch's time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -146,8 +146,8 @@ __device__ __forceinline__ void join_row(float& sum, float& top) {
 // high + low, that is off by 2^-45 of it (2^-30 where the row's largest number lies near f32's, because low is subnormal then), and
 // v * high + (v * low) is one product and one fused multiply-add, rounded once: a quotient that f32 holds is exact, and no other is off by more than half a step
 // and 2^-30 of it. `high` lies a little below, so that `low` is positive and a zero keeps its sign.
-// (Calls behind one another, so / with the product alone: 4096 x 14336 bf16 32.7 / 31.6 us; 8192 x 8192 f16 norm with residual 76.1 / 76.0; 1023 x 5003 bf16 norm,
-// element by element, 9.7 / 9.1.)
+// (Calls behind one another from cold memory, so / with the product alone: 4096 x 14336 bf16 32.7 / 31.6 us; 8192 x 8192 f16 norm with residual 76.1 / 76.0;
+// 1023 x 5003 bf16 norm, element by element, 9.7 / 9.1.)
 template <bool NORM, bool E4M3>
 struct Factor {
     float lift, high, low;
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rows_in_registers(const R
 }
 
 // Rows that start at no vector boundary, or whose width is no whole number of vectors, up to EACH * 512 elements: a block per
-// row, element by element, one read of the row. Bound by its instructions (1023 x 5003 bf16 to e4m3: 8.7 us, 1.8 TB/s; reading twice 14.3).
+// row, element by element, one read of the row. Bound by its instructions (1023 x 5003 bf16 to e4m3: 9.7 us, 1.6 TB/s).
 constexpr int EACH = 16;
 template <class T, bool NORM, bool RESIDUAL, bool E4M3>
 __global__ void __launch_bounds__(512) rows_by_element(const Rows p) {

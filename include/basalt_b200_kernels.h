@@ -181,10 +181,11 @@ enum { BASALT_K_TYPE_F16 = 0, BASALT_K_TYPE_BF16 = 1, BASALT_K_TYPE_F32 = 2 };
  *   scales[r] = max(max_k |y_k| / 448, 2^-126),   y stored as e4m3(y_k / scales[r]), to the nearest, ties to even;
  * the quotient is an f32 one by the stored scale: exact where f32 holds it, else off by no more than half a step and 2^-30 of it (y is not
  * rounded before it).
- * The norm goes by h before its rounding to total.  An infinity or a NaN in a row gives what the formulas give; no other
+ * The norm goes by h before its rounding to total.  The squares, their sum and h * weight are f32, too: a row whose |h| reaches
+ * 2^64 has an infinite mean and a y of zeros.  An infinity or a NaN in a row gives what the formulas give; no other
  * row is touched by it.  An output may be an input's own buffer of the same stride and type (total = residual, y = x); any
- * other overlap is refused.  Any alignment and width is right; 16-byte aligned rows of whole 16-byte pieces are read
- * once, others twice.  rows = 0 does nothing.  Pointers must lie on the current device. */
+ * other overlap is refused.  Any alignment and width is right.  Rows of whole 16-byte pieces from aligned starts are read once up to
+ * 32768 elements (16384 in f32), others up to 8192; longer ones twice.  rows = 0 does nothing.  Pointers must lie on the current device. */
 int basalt_k_rms_norm(int type, const void *x, int64_t ldx, const void *residual, int64_t ldr, void *total, int64_t ldt,
                       const void *weight, float eps, void *y, int64_t ldy, float *scales, int64_t rows, int64_t cols,
                       void *stream);
@@ -195,11 +196,11 @@ int basalt_k_quantize_e4m3(int type, const void *x, int64_t ldx, void *q, int64_
                            int64_t cols, void *stream);
 
 /* C[m, n] = (sum_k A[m, k] * B[n, k]) * a_scales[m] * b_scales[n]: A [M x K] and B [N x K] (weights, one row per output
- * channel) are e4m3, the sums f32 on tcgen05 tensor cores, C [M x N] is of c_type (F16, BF16, F32), rounded once.  Any M, N, K >= 1
+ * channel) are e4m3, the sums f32 on tcgen05 tensor cores (which truncate them, some 9e-11 of the result for each k), C [M x N] is of c_type
+ * (F16, BF16, F32), rounded once, but for f32 with K beyond 8192: that goes in several launches whose results are added to C in turn.  Any M, N, K >= 1
  * (M or N 0 does nothing); A, B, lda and ldb must be multiples of 16 bytes (pad the rows: bytes
  * beyond K are not read), C and ldc need their element's alignment only.  Rows and columns beyond M and N are left as
- * they were.  No workspace, no atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16.
- * Into f32, a K beyond 8192 goes in several launches whose results are added to C in turn. */
+ * they were.  No workspace, no atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16. */
 int basalt_k_matmul_e4m3(const void *A, int64_t lda, const float *a_scales, const void *B, int64_t ldb,
                          const float *b_scales, int c_type, void *C, int64_t ldc, int M, int N, int K, int32_t *status,
                          void *stream);
@@ -209,7 +210,8 @@ int basalt_k_matmul_e4m3(const void *A, int64_t lda, const float *a_scales, cons
  * ceil(K / group)] of `type` and zeros z [N x ceil(K / group)] (one byte each, 0 .. 128; NULL: 8 everywhere), both
  * without gaps, from a multiple of 4 bytes.  group is a multiple of 32.  Any M, N, K >= 1 (M or N 0 does nothing); X, W and
  * ldw must be multiples of 16 bytes, ldx of 8 elements.  Sums are f32 and C is rounded once.  Up to 16 rows (M) nothing
- * else is rounded; beyond, a weight (q - z) * s may be rounded to `type` before the product, which must not overflow it.
+ * else is rounded; beyond, a weight (q - z) * s may be rounded to `type` before the product, which must not overflow it (the error of C
+ * grows by a third, so 16 and 17 rows of one batch may differ in their last bits).
  * Bytes beyond a row's K values are not read; rows and columns beyond M and N are left as they were.  No workspace, no
  * atomics: the same call gives the same bits.  `status` as for basalt_k_matmul_f16. */
 int basalt_k_matmul_w4(int type, const void *X, int64_t ldx, const void *W, int64_t ldw, const void *scales,

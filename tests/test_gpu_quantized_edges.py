@@ -62,6 +62,26 @@ def test_norm_to_e4m3_of_the_largest_weights(gpu, cols):
     check_e4m3(down(dy, y), down(ds, s), want, (cols / 2 + 10) * U)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_norm_of_rows_whose_squares_exceed_f32_is_zero(gpu, cols, t):
+    """Their mean is infinite in f32; the rows beside them are what they are alone."""
+    x = rows(gen(cols), 4, cols, T[t])
+    x[1], x[2, cols - 1] = -torch.finfo(T[t]).max, 2.0 ** 64
+    for out8 in (False, True):
+        got = []
+        for v in (x, x[[0, 3]]):
+            n = v.shape[0]
+            y, s = torch.full((n, cols), 0x55, dtype=torch.uint8) if out8 else torch.full((n, cols), 7.0, dtype=T[t]), torch.full((n,), 5.0)
+            dy, ds = up(gpu, y), up(gpu, s)
+            kernels.rms_norm(up(gpu, v.contiguous()), dy, n, cols, t, scales=ds if out8 else None)
+            gpu.synchronize()
+            got.append((down(dy, y), down(ds, s)))
+        (y, s), (alone, s_alone) = got
+        assert torch.equal(y[[0, 3]], alone) and torch.equal(s[[0, 3]], s_alone)
+        assert ((y[1:3] & 0x7F if out8 else y[1:3]) == 0).all() and (not out8 or (s[1:3] == 2.0 ** -126).all())
+
+
 def e4m3_of_the_quotient(y, s):
     """y / s in f32, as the CPU divides, then e4m3 to the nearest, ties to even."""
     return (y.float() / s[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
