@@ -48,7 +48,7 @@ __device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.a
 // through the async proxy, which an arrival on a barrier alone does not order against plain reads: without this, reads that queued behind the copies' cache
 // misses saw the next slab (14720 -> 14931 in groups of 32, bf16, from cold memory, with a warp that only carries scales: one launch in four missed 32 k of X
 // in the rows of a warp on that warp's scheduler).
-// It costs 0.5 us of 20.5 for 17 rows through 8192 x 8192, nothing that shows for one row.
+// It costs 0.6 us of 20.5 for 17 rows through 8192 x 8192, nothing that shows for one row.
 __device__ __forceinline__ void reads_done() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A slab's scales and zero points in shared memory: of each of the tile's 128 rows the groups that 256 k touch, at most 8 / FLUSH where
